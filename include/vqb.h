@@ -383,6 +383,134 @@ vqb_status vqb_ep_combine(const vqb_ep_layout* layout, void* const* regions, con
 vqb_status vqb_ep_reduce(const vqb_ep_layout* layout, void* region, void* y, vqb_dtype y_dtype, int32_t n_tokens,
                          vqb_stream_t stream);
 
+/* ---- The attention part of a served layer: paged cache, rotary positions, attention ----
+ *
+ * No reference counterpart (the reference's host library supplies attention);
+ * these calls are what a layer needs between its q / k / v projections and its
+ * output projection.  Keys and values live in a pool of pages
+ * [num_pages, kv_heads, page_size, head_dim]; a request's block table row
+ * lists its pages, and a token's slot is page * page_size + its offset in the
+ * page.  Tokens that a whole batch shares (a prefix) sit in pages of their own,
+ * listed once for the call; a request's table holds its own tokens only, so
+ * the prefix may end anywhere in its last page. */
+
+/* One step's block tables and slot map, built on the device from the
+ * requests' lengths, in one launch.
+ *
+ * Request r holds context_lens[r] tokens and gets new_lens[r] more;
+ * new_lens[r] == -1 says that it has finished and gives its pages back (its
+ * row becomes -1, its length 0).  Free pages wait in a ring: page
+ * free_pages[i % ring_size] for i from state[0] up to state[1].  Pages given
+ * back go to the ring's end in the order of requests and of their pages, then
+ * requests take what they lack from its start in the order of requests.  A
+ * request that needs more pages than its row has places, or than are left at
+ * its turn (the needs of all before it counted), is refused: its row and its
+ * length stay, its new tokens get slot -1, and so does every later one that
+ * lacks a page.
+ *
+ * Results: block_table_out (unused places -1), kv_lens (tokens held after the
+ * step), cu_q [n_requests + 1] (where each request's new tokens start among all
+ * new tokens), and for each of max_tokens places slots, positions
+ * (position_offset + the token's place in its request) and requests; places
+ * past the last token get -1, 0, -1.  state_out = {start, end, requests
+ * refused, 0}.  Every out pointer may be its in pointer (the update is then in
+ * place, kv_lens over context_lens; unused places of a row that is kept stay as they are): a
+ * captured step can replay.  state[3] counts the call's blocks and is 0
+ * between calls; calls with one state must not overlap.
+ * n_requests <= 8192, page_size >= 1. */
+typedef struct vqb_paged_desc {
+  int32_t n_requests;
+  int32_t table_width;        /* places of a block table row (its stride) */
+  int32_t page_size;
+  int32_t ring_size;          /* places of the ring of free pages */
+  int32_t max_tokens;         /* places of slots / positions / requests */
+  int32_t position_offset;    /* tokens before every request's own: the shared prefix's length */
+} vqb_paged_desc;
+
+vqb_status vqb_paged_tables(const vqb_paged_desc* desc, const int32_t* context_lens, const int32_t* new_lens,
+                            const int32_t* block_table, const int32_t* free_pages, int64_t* state,
+                            int32_t* block_table_out, int32_t* free_pages_out, int64_t* state_out, int32_t* kv_lens,
+                            int32_t* cu_q, int32_t* slots, int32_t* positions, int32_t* requests,
+                            vqb_stream_t stream);
+
+/* Rotary positions, and the step's keys and values into the paged cache, in
+ * one launch.  The first rotary_dim elements of each head of q and k are
+ * rotated in pairs: (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t)
+ * with t = 2 pi * positions[n] * freq[i] / 2^64 for pair i: freq [rotary_dim / 2]
+ * holds turns per position as fixed point, so that the angle is reduced
+ * exactly by integer arithmetic at any position.  interleaved: pair i is
+ * elements (2i, 2i + 1); else (i, i + rotary_dim / 2).  Rotated q goes to
+ * q_out (which may be q), rotated k and plain v to the cache at slots[n]; a
+ * slot outside the pool is not stored.  kv_heads = 0 rotates q alone (k, v,
+ * caches and slots unused).  Strides are in elements; the elements of a head are
+ * contiguous.  dtype fp16 / bf16, arithmetic fp32, one rounding. */
+typedef struct vqb_rotary_desc {
+  int32_t n_tokens;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;           /* even */
+  int32_t rotary_dim;         /* even, <= head_dim */
+  int32_t interleaved;
+  int32_t page_size;
+  int32_t num_pages;
+  float amplitude;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int64_t kc_page_stride, kc_head_stride, kc_token_stride;
+  int64_t vc_page_stride, vc_head_stride, vc_token_stride;
+} vqb_rotary_desc;
+
+vqb_status vqb_rotary_append(const vqb_rotary_desc* desc, vqb_dtype dtype, const void* q, const void* k, const void* v,
+                             const int32_t* positions, const int64_t* freq, const int32_t* slots, void* q_out,
+                             void* k_cache, void* v_cache, vqb_stream_t stream);
+
+/* Attention of a batch over the paged cache.  Request r's queries are rows
+ * cu_q[r] .. cu_q[r+1] of q [n_tokens, heads, head_dim]; it holds kv_lens[r]
+ * tokens of its own, its queries being the last of them.  Query i of n sees
+ * the whole prefix and its own tokens up to kv_lens[r] - n + i (all of them
+ * when causal is 0).  Query head h reads key / value head
+ * h / (heads / kv_heads).  out = softmax(scale * q k^T) v with scores,
+ * softmax and sums in fp32, rounded once to dtype; a row that sees nothing is 0.
+ * lse (optional, fp32 [n_tokens, heads]): log of the sum of exp of the scaled
+ * scores (-inf for such a row).  Rows past cu_q[n_requests] are not written.
+ * Cache places past a request's length are never used, whatever they hold; a
+ * page outside the pool reads as zeros.
+ *
+ * max_q_len / max_kv_len bound the requests' queries and own tokens (the
+ * lengths themselves are on the device): what lies past them is left out.
+ * page_size a power of two, 16 to 1024; head_dim 64 or 128; dtype fp16 / bf16;
+ * strides in elements, multiples of 8, the elements of a head contiguous; q,
+ * caches and out 16-byte aligned.  The first 16 bytes of the workspace are a status
+ * block the call rewrites (int32 [1] = VQB_TIMEOUT when a bounded device wait
+ * gave up). */
+typedef struct vqb_attention_desc {
+  int32_t n_requests;
+  int32_t n_tokens;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t table_width;
+  int32_t max_q_len;
+  int32_t max_kv_len;
+  int32_t prefix_len;
+  int32_t causal;
+  float scale;
+  int64_t q_token_stride, q_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int64_t kc_page_stride, kc_head_stride, kc_token_stride;
+  int64_t vc_page_stride, vc_head_stride, vc_token_stride;
+} vqb_attention_desc;
+
+size_t vqb_prefix_attention_workspace_size(const vqb_attention_desc* desc);
+vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_dtype dtype, const void* q, const void* k_cache,
+                                const void* v_cache, const int32_t* block_table, const int32_t* kv_lens,
+                                const int32_t* cu_q, const int32_t* prefix_pages, void* out, float* lse,
+                                void* workspace, size_t workspace_bytes, vqb_stream_t stream);
+
 /* Measurement aids; neither has a counterpart in the reference, whose Metal
  * runtime exposes no launch accounting or per-kernel timing.
  *

@@ -87,6 +87,31 @@ class EpOptions(ctypes.Structure):
     _fields_ = [("phases", ctypes.c_int32), ("wait_limit_us", ctypes.c_int32)]
 
 
+class PagedDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_requests", "table_width", "page_size", "ring_size", "max_tokens",
+                                              "position_offset")]
+
+
+_CACHE_STRIDES = [(n, ctypes.c_int64) for n in ("kc_page_stride", "kc_head_stride", "kc_token_stride",
+                                                "vc_page_stride", "vc_head_stride", "vc_token_stride")]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_tokens", "heads", "kv_heads", "head_dim", "rotary_dim",
+                                              "interleaved", "page_size", "num_pages")] + [
+        ("amplitude", ctypes.c_float)] + [(n, ctypes.c_int64) for n in (
+            "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride",
+            "out_token_stride", "out_head_stride")] + _CACHE_STRIDES
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_requests", "n_tokens", "heads", "kv_heads", "head_dim", "page_size",
+                                              "num_pages", "table_width", "max_q_len", "max_kv_len", "prefix_len",
+                                              "causal")] + [("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride", "out_token_stride",
+                                      "out_head_stride")] + _CACHE_STRIDES
+
+
 VQB_EP_MAX_WORLD = 8
 VQB_EP_STATUS_OFFSET = 272
 VQB_EP_IPC_HANDLE_BYTES = 64
@@ -145,6 +170,14 @@ def _bind(L):
     L.vqb_dense_mlp_workspace_size.argtypes = [P, i32]
     L.vqb_dense_mlp_forward.restype = i32
     L.vqb_dense_mlp_forward.argtypes = [P, P, i32, i32, P, P, sz, P, P]
+    L.vqb_paged_tables.restype = i32
+    L.vqb_paged_tables.argtypes = [P] * 15
+    L.vqb_rotary_append.restype = i32
+    L.vqb_rotary_append.argtypes = [P, i32] + [P] * 10
+    L.vqb_prefix_attention_workspace_size.restype = sz
+    L.vqb_prefix_attention_workspace_size.argtypes = [P]
+    L.vqb_prefix_attention.restype = i32
+    L.vqb_prefix_attention.argtypes = [P, i32] + [P] * 10 + [sz, P]
     L.vqb_ep_region_bytes.restype = sz
     L.vqb_ep_region_bytes.argtypes = [P, P]
     L.vqb_ep_region_alloc.restype = i32
@@ -212,7 +245,8 @@ def exported_symbols():
             "vqb_moe_block_workspace_size", "vqb_moe_block_forward", "vqb_dense_mlp_supported",
             "vqb_dense_mlp_workspace_size", "vqb_dense_mlp_forward", "vqb_ep_region_bytes", "vqb_ep_region_alloc", "vqb_ep_region_free",
             "vqb_ep_ipc_handle", "vqb_ep_ipc_open", "vqb_ep_ipc_close", "vqb_ep_dispatch", "vqb_ep_combine",
-            "vqb_ep_reduce"]
+            "vqb_ep_reduce", "vqb_paged_tables", "vqb_rotary_append", "vqb_prefix_attention_workspace_size",
+            "vqb_prefix_attention"]
 
 
 def launch_count() -> int:

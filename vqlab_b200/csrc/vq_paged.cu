@@ -1,0 +1,296 @@
+// vqb_paged_tables: one step's block tables, lengths and slot map from the
+// requests' lengths.
+//
+// The mathematics is three running sums over the requests r (context c, new n,
+// page size P): pages given back (n = -1: ceil(c / P)), new tokens, and pages
+// needed (ceil((c + n) / P) - ceil(c / P)).  With them every output element has
+// a closed form: request r's j-th new page is entry (start + need sum before r
+// + j) of the ring of free pages, extended by the pages given back in this
+// call, and token t belongs to the request whose token sum covers it.  So no
+// element waits for another: every block computes the sums itself (a few
+// thousand integers out of L2, about a microsecond) and then writes its share
+// of the rows and tokens -- one launch and no grid-wide step.  In-place calls
+// are safe because the only values a block may still read that the call
+// overwrites (lengths, state, the rows of finished requests) are written by
+// the block that arrives last.
+//
+// Bound: bytes (table rows in and out, 12 bytes a token); small steps are
+// bound by the launch and the sums' latency.
+#include "vqb_common.cuh"
+#include "vqb_internal.h"
+
+namespace vqb {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kMaxRequests = 8192;
+
+struct PagedParams {
+  vqb_paged_desc d;
+  const int32_t* context;
+  const int32_t* fresh;
+  const int32_t* table_in;
+  const int32_t* ring_in;
+  int64_t* state;
+  int32_t* table;
+  int32_t* ring;
+  int64_t* state_out;
+  int32_t* kv_lens;
+  int32_t* cu_q;
+  int32_t* slots;
+  int32_t* positions;
+  int32_t* requests;
+};
+
+// What request r holds and wants; lengths below zero count as zero and a row
+// never holds more pages than it has places.
+struct Request {
+  int held;    // pages of its row in use
+  int tokens;  // new tokens
+  int need;    // pages it lacks
+  int back;    // pages it gives back
+  bool fits;   // its row has places enough
+};
+
+__device__ __forceinline__ Request load_request(const PagedParams& p, int r) {
+  const int c = max(__ldcg(p.context + r), 0), n = __ldcg(p.fresh + r);
+  const int P = p.d.page_size;
+  Request q;
+  q.held = min(c > 0 ? (c - 1) / P + 1 : 0, p.d.table_width);
+  q.tokens = max(n, 0);
+  const int64_t pages = (static_cast<int64_t>(c) + q.tokens + P - 1) / P;
+  q.fits = pages <= p.d.table_width;
+  q.need = n < 0 || !q.fits ? 0 : max(static_cast<int>(pages) - q.held, 0);
+  q.back = n < 0 ? q.held : 0;
+  return q;
+}
+
+// The last index in [0, n) whose sum is <= v (sums[0] = 0, non-decreasing).
+__device__ __forceinline__ int find(const int* sums, int n, int v) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sums[mid] <= v) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kThreads) paged_tables_kernel(PagedParams p) {
+  extern __shared__ int s_sums[];
+  const int R = p.d.n_requests;
+  int* s_tok = s_sums;               // [R + 1] new tokens before r
+  int* s_need = s_tok + R + 1;       // [R + 1] pages needed before r
+  int* s_back = s_need + R + 1;      // [R + 1] pages given back before r
+  __shared__ int s_warp[3][kThreads / 32];
+  __shared__ int s_refused, s_given, s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_trigger();
+  if (tid == 0) {
+    s_refused = 0;
+    s_given = 0;
+  }
+
+  // ---- the three sums: a thread adds up a run of requests, then the threads' totals are scanned
+  const int per = (R + kThreads - 1) / kThreads;
+  const int r0 = min(tid * per, R), r1 = min(r0 + per, R);
+  int tot[3] = {0, 0, 0};
+  for (int r = r0; r < r1; ++r) {
+    const Request q = load_request(p, r);
+    tot[0] += q.tokens;
+    tot[1] += q.need;
+    tot[2] += q.back;
+  }
+  int inc[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    inc[k] = tot[k];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc[k], o);
+      if (lane >= o) inc[k] += v;
+    }
+    if (lane == 31) s_warp[k][warp] = inc[k];
+  }
+  __syncthreads();
+  if (warp < 3) {
+    int v = lane < kThreads / 32 ? s_warp[warp][lane] : 0;
+    const int mine = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane < kThreads / 32) s_warp[warp][lane] = v - mine;
+  }
+  __syncthreads();
+  {
+    int at[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) at[k] = s_warp[k][warp] + inc[k] - tot[k];
+    for (int r = r0; r < r1; ++r) {
+      const Request q = load_request(p, r);
+      s_tok[r] = at[0];
+      s_need[r] = at[1];
+      s_back[r] = at[2];
+      at[0] += q.tokens;
+      at[1] += q.need;
+      at[2] += q.back;
+    }
+    if (r1 == R && (r0 < R || tid == 0)) {  // the thread with the last request (thread 0 when there is none)
+      s_tok[R] = at[0];
+      s_need[R] = at[1];
+      s_back[R] = at[2];
+    }
+  }
+  __syncthreads();
+
+  const int64_t head = __ldcg(p.state), tail = __ldcg(p.state + 1);
+  const uint32_t F = static_cast<uint32_t>(p.d.ring_size);
+  const int returned = s_back[R];
+  const int64_t avail = tail + returned - head;
+  const uint32_t head_mod = static_cast<uint32_t>(static_cast<uint64_t>(head) % F);
+  const uint32_t tail_mod = static_cast<uint32_t>(static_cast<uint64_t>(tail) % F);
+  const int64_t waiting = tail - head;  // entries of the ring before this call's returns
+  const int W = p.d.table_width, P = p.d.page_size;
+  auto taken = [&](int r, const Request& q) {
+    return q.fits && (q.need == 0 || static_cast<int64_t>(s_need[r]) + q.need <= avail);
+  };
+  // entry `i` from the ring's start: a free page, or one given back in this call
+  auto page_at = [&](int i) -> int {
+    if (i < waiting) return __ldcg(p.ring_in + (head_mod + static_cast<uint32_t>(i)) % F);
+    const int b = i - static_cast<int>(waiting);
+    if (b < 0 || b >= returned) return -1;
+    // the last request whose sum is <= b gives it back: those after it with the same sum give nothing
+    const int r = find(s_back, R, b);
+    return __ldcg(p.table_in + static_cast<int64_t>(r) * W + (b - s_back[r]));
+  };
+  const bool table_in_place = p.table == p.table_in, ring_in_place = p.ring == p.ring_in;
+  const int gwarp = blockIdx.x * (kThreads / 32) + warp, gwarps = gridDim.x * (kThreads / 32);
+  const int64_t gthread = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
+  const int64_t gthreads = static_cast<int64_t>(gridDim.x) * kThreads;
+
+  // ---- table rows and pages given back, a warp to a request
+  for (int r = gwarp; r < R; r += gwarps) {
+    const Request q = load_request(p, r);
+    const bool gone = __ldcg(p.fresh + r) < 0;
+    const bool ok = !gone && taken(r, q);
+    const int32_t* in = p.table_in + static_cast<int64_t>(r) * W;
+    int32_t* out = p.table + static_cast<int64_t>(r) * W;
+    if (gone) {
+      for (int j = lane; j < q.held; j += 32)
+        p.ring[(tail_mod + static_cast<uint32_t>(s_back[r] + j)) % F] = __ldcg(in + j);
+    }
+    const int keep = gone ? 0 : q.held, end = ok ? q.held + q.need : keep;
+    if (table_in_place) {
+      for (int j = keep + lane; j < end; j += 32) out[j] = page_at(s_need[r] + j - q.held);
+    } else {
+      for (int j = lane; j < W; j += 32)
+        out[j] = j < keep ? __ldcg(in + j) : (j < end ? page_at(s_need[r] + j - q.held) : -1);
+    }
+  }
+  // the ring's other places (those given back in this call were written above)
+  if (!ring_in_place) {
+    for (int64_t i = gthread; i < F; i += gthreads) {
+      const uint32_t from_tail = (static_cast<uint32_t>(i) + F - tail_mod) % F;
+      if (from_tail >= static_cast<uint32_t>(returned)) p.ring[i] = __ldcg(p.ring_in + i);
+    }
+  }
+  // ---- tokens
+  const int total = s_tok[R];
+  for (int64_t t = gthread; t < p.d.max_tokens; t += gthreads) {
+    int slot = -1, pos = 0, r = -1;
+    if (t < total) {
+      r = find(s_tok, R, static_cast<int>(t));
+      const Request q = load_request(p, r);
+      const int place = max(__ldcg(p.context + r), 0) + static_cast<int>(t) - s_tok[r];
+      pos = p.d.position_offset + place;
+      if (taken(r, q)) {
+        const int col = place / P;
+        const int page = col < q.held ? __ldcg(p.table_in + static_cast<int64_t>(r) * W + col)
+                                      : page_at(s_need[r] + col - q.held);
+        if (page >= 0) slot = page * P + place % P;
+      }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+    p.requests[t] = r;
+  }
+
+  // ---- the block that arrives last has no reader left beside it
+  __syncthreads();
+  if (tid == 0) {
+    __threadfence();
+    const unsigned long long n = atomicAdd(reinterpret_cast<unsigned long long*>(p.state + 3), 1ull);
+    s_last = n == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  int refused = 0, given = 0;
+  for (int r = tid; r < R; r += kThreads) {
+    const Request q = load_request(p, r);
+    const bool gone = __ldcg(p.fresh + r) < 0;
+    const bool ok = !gone && taken(r, q);
+    const int c = max(__ldcg(p.context + r), 0);
+    if (!gone && !ok) ++refused;
+    if (ok) given += q.need;
+    p.kv_lens[r] = gone ? 0 : (ok ? c + q.tokens : c);
+  }
+  for (int r = tid; r <= R; r += kThreads) p.cu_q[r] = s_tok[r];
+  if (refused) atomicAdd(&s_refused, refused);
+  if (given) atomicAdd(&s_given, given);
+  if (table_in_place) {
+    for (int r = warp; r < R; r += kThreads / 32) {
+      const int back = s_back[r + 1] - s_back[r];
+      for (int j = lane; j < back; j += 32) p.table[static_cast<int64_t>(r) * W + j] = -1;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    p.state[3] = 0;
+    p.state_out[0] = head + s_given;
+    p.state_out[1] = tail + returned;
+    p.state_out[2] = s_refused;
+    p.state_out[3] = 0;
+  }
+}
+
+}  // namespace
+}  // namespace vqb
+
+using namespace vqb;
+
+extern "C" vqb_status vqb_paged_tables(const vqb_paged_desc* desc, const int32_t* context_lens, const int32_t* new_lens,
+                                       const int32_t* block_table, const int32_t* free_pages, int64_t* state,
+                                       int32_t* block_table_out, int32_t* free_pages_out, int64_t* state_out,
+                                       int32_t* kv_lens, int32_t* cu_q, int32_t* slots, int32_t* positions,
+                                       int32_t* requests, vqb_stream_t stream) {
+  if (!desc) return VQB_NULL_POINTER;
+  const vqb_paged_desc& d = *desc;
+  if (d.n_requests < 0 || d.table_width < 1 || d.page_size < 1 || d.ring_size < 1 || d.max_tokens < 0)
+    return VQB_BAD_SHAPE;
+  if (d.n_requests > kMaxRequests) return VQB_UNSUPPORTED_GEOMETRY;
+  if (!free_pages || !state || !free_pages_out || !state_out || !cu_q) return VQB_NULL_POINTER;
+  if (d.n_requests > 0 && (!context_lens || !new_lens || !block_table || !block_table_out || !kv_lens))
+    return VQB_NULL_POINTER;
+  if (d.max_tokens > 0 && (!slots || !positions || !requests)) return VQB_NULL_POINTER;
+  DeviceInfo di;
+  if (device_info(&di) != VQB_OK) return VQB_CUDA_ERROR;
+  PagedParams p{d, context_lens, new_lens, block_table, free_pages, state, block_table_out, free_pages_out, state_out,
+                kv_lens, cu_q, slots, positions, requests};
+  // a block for every 16 rows (one a warp) or 512 tokens or ring places, one block an SM at most
+  int64_t blocks = (static_cast<int64_t>(d.n_requests) + kThreads / 32 - 1) / (kThreads / 32);
+  const int64_t others = (static_cast<int64_t>(d.max_tokens) + kThreads - 1) / kThreads;
+  const int64_t places = block_table == block_table_out ? 0 : (static_cast<int64_t>(d.ring_size) + kThreads - 1) / kThreads;
+  blocks = blocks > others ? blocks : others;
+  blocks = blocks > places ? blocks : places;
+  blocks = blocks < 1 ? 1 : (blocks > di.sms ? di.sms : blocks);
+  const size_t smem = 3 * sizeof(int) * (static_cast<size_t>(d.n_requests) + 1);
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(paged_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem)) != cudaSuccess)
+    return VQB_CUDA_ERROR;
+  if (launch_pdl(paged_tables_kernel, static_cast<unsigned>(blocks), kThreads, smem,
+                 reinterpret_cast<cudaStream_t>(stream), p) != cudaSuccess)
+    return VQB_CUDA_ERROR;
+  note_launch();
+  return VQB_OK;
+}
