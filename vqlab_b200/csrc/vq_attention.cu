@@ -1,143 +1,169 @@
 // vqb_prefix_attention: attention of a batch over the paged cache.
 //
-// o = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q.k_j - m) in one pass over
-// the keys: m is a running maximum, and what has been summed is scaled by
-// exp(m_old - m_new) when it moves.
-//
-// A warp takes one (query, head) row and 32 keys at a time: a lane computes the
-// score of one key, then the lanes share the value's dimensions.
-#include "vqb_common.cuh"
-#include "vqb_internal.h"
+// o = sum_j p_j v_j / sum_j p_j with p_j = 2^(s_j - m), s_j = scale log2(e) q.k_j,
+// in one pass over the keys with a running maximum.  Sums over disjoint sets of
+// a row's keys join exactly: with partial (m_i, l_i, O_i) and M = max m_i,
+// o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  So a call is a list of passes
+// over parts of the keys, and a join when there are several partial results:
+//   * rows of all requests together over the shared prefix
+//     (vq_attention_tiles.cu): its pages are read once for 256 rows;
+//   * each request's own keys: vq_attention_decode.cu for up to 16 rows a
+//     key/value head, vq_attention_tiles.cu for more;
+//   * both over splits of the keys where there are fewer blocks than SMs.
+#include "vq_attention.cuh"
 
 namespace vqb {
 namespace {
 
-struct AttnParams {
-  vqb_attention_desc d;
-  const uint16_t* q;
-  const uint16_t* kc;
-  const uint16_t* vc;
-  const int32_t* table;
-  const int32_t* kv_lens;
-  const int32_t* cu_q;
-  const int32_t* prefix_pages;
-  uint16_t* out;
-  float* lse;
-  int group;
-  int page_shift;
-  float scale_log2;  // scale * log2(e): scores in powers of two
+struct AttnPlan {
+  AttnPass shared;     // splits = 0: no pass over the prefix alone
+  AttnPass own;
+  bool decode;         // the own pass runs the decode kernel
+  unsigned shared_tiles, own_tiles;
+  int parts;           // partial results; 0: the own pass writes out
 };
 
-template <bool BF16>
-__device__ __forceinline__ float widen(uint16_t h) {
-  if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(h) << 16);
-  else return __half2float(__ushort_as_half(h));
-}
-template <bool BF16>
-__device__ __forceinline__ uint16_t narrow(float v) {
-  if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
-  else return __half_as_ushort(__float2half_rn(v));
-}
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The request whose queries include token n: the last r with cu_q[r] <= n (n < cu_q[R]).
-__device__ __forceinline__ int request_of(const int32_t* cu_q, int R, int n) {
-  int lo = 0, hi = R - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(cu_q + mid) <= n) lo = mid;
-    else hi = mid - 1;
+// How many splits of `tiles` key tiles (a tile costs one) finish first: rounds
+// of blocks over the SMs times the longest block (its tiles and about three
+// tiles' worth of start and end), and the join's traffic (`row_cost`: partial
+// result of one split, in tiles).
+int pick_splits(int64_t blocks, int64_t tiles, int slots, double row_cost, bool joined_anyway) {
+  int best = 1;
+  double best_t = 1e30;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const double rounds = static_cast<double>(ceil_div(blocks * s, slots));
+    double t = rounds * (static_cast<double>(ceil_div(tiles, s)) + 3.0);
+    if (s > 1 || joined_anyway) t += row_cost * s + 3.0;
+    if (t < best_t * 0.98) {
+      best_t = t;
+      best = s;
+    }
   }
-  return lo;
+  return best;
 }
 
-template <bool BF16, int D>
-__global__ void __launch_bounds__(256) attention_rows_kernel(AttnParams p) {
-  __shared__ float s_q[8][D];
+AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
+  AttnPlan a{};
+  const int group = d.heads / d.kv_heads;
+  const int64_t rows = static_cast<int64_t>(d.n_tokens) * group;  // of one key/value head
+  const int64_t most = static_cast<int64_t>(d.max_q_len < d.n_tokens ? d.max_q_len : d.n_tokens) * group;
+  a.decode = most <= 16;
+  // the prefix for all rows at once, unless a request fills tiles by itself
+  const bool joint = d.prefix_len > 0 && d.n_requests > 1 && most <= 256;
+  // a partial result's bytes over the time of a key tile (about 1 us at 4 TB/s)
+  const double row_cost = static_cast<double>(d.n_tokens) * d.heads * d.head_dim * 8.0 / 4.0e6;
+  if (joint) {
+    a.shared_tiles = static_cast<unsigned>(ceil_div(rows, 256));
+    a.shared = AttnPass{1, 0, pick_splits(static_cast<int64_t>(a.shared_tiles) * d.kv_heads, ceil_div(d.prefix_len, 128),
+                                          sms, row_cost, true), 0, 0};
+  }
+  const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
+  a.own.prefix = !joint && d.prefix_len > 0;
+  if (a.decode) {
+    // a block streams 256 keys or more; about two rounds of two blocks an SM
+    const int64_t blocks = static_cast<int64_t>(d.n_requests) * d.kv_heads;
+    int64_t s = ceil_div(4 * sms, blocks);
+    if (s > ceil_div(keys, 256)) s = ceil_div(keys, 256);
+    if (s > 64) s = 64;
+    if (s < 1) s = 1;
+    a.own.chunk = static_cast<int>(ceil_div(ceil_div(keys, s), 64) * 64);
+    if (a.own.prefix) a.own.chunk += 64;  // the prefix and the own keys start groups of their own
+    if (a.own.chunk < 64) a.own.chunk = 64;
+    a.own.splits = static_cast<int>(s);
+  } else {
+    a.own_tiles = static_cast<unsigned>(rows / 256 + d.n_requests);
+    const int64_t blocks = (rows / 256 > d.n_requests ? rows / 256 : d.n_requests) * d.kv_heads;
+    a.own.splits = pick_splits(blocks, ceil_div(keys, 128), sms, row_cost, joint);
+  }
+  a.parts = a.shared.splits + a.own.splits;
+  a.own.part0 = a.shared.splits;
+  if (a.parts == 1) {
+    a.own.part0 = -1;
+    a.parts = 0;
+  }
+  return a;
+}
+
+constexpr size_t kStatusBytes = 256;
+
+size_t part_rows(const vqb_attention_desc& d) { return static_cast<size_t>(d.n_tokens) * d.heads; }
+size_t ml_bytes(const vqb_attention_desc& d, int parts) { return (parts * part_rows(d) * sizeof(float2) + 255) & ~size_t(255); }
+
+// Joins a row's partial results, a warp a row.  Bound: the partial results'
+// bytes, which are in L2 as a rule.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, int parts) {
   pdl_wait();
   pdl_trigger();
   const vqb_attention_desc& d = p.d;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + warp;
-  const int n = static_cast<int>(row / d.heads), h = static_cast<int>(row - static_cast<int64_t>(n) * d.heads);
-  if (n >= d.n_tokens || n >= __ldg(p.cu_q + d.n_requests)) return;
-  const int r = request_of(p.cu_q, d.n_requests, n);
-  const int q0 = __ldg(p.cu_q + r), nq = __ldg(p.cu_q + r + 1) - q0;
-  int len = max(min(__ldg(p.kv_lens + r), d.max_kv_len), 0);
-  len = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(d.table_width) << p.page_shift));
-  const int seen = d.causal ? max(min(len - nq + (n - q0) + 1, len), 0) : len;
-  const int kvh = h / p.group;
-  const uint16_t* q = p.q + n * d.q_token_stride + h * d.q_head_stride;
-  for (int e = lane; e < D; e += 32) s_q[warp][e] = widen<BF16>(q[e]);
-  __syncwarp();
-
-  float m = -INFINITY, l = 0.0f, acc[D / 32];
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = static_cast<int64_t>(d.n_tokens) * d.heads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int64_t n = row / d.heads;
+  const int h = static_cast<int>(row - n * d.heads);
+  if (n >= __ldg(p.cu_q + d.n_requests)) return;
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(p.part_ml + i * rows + row).x);
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float base = m == -INFINITY ? 0.0f : m;
+  constexpr int kPer = D / 32;
+  float acc[kPer], l = 0.0f;
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
-  for (int part = 0; part < 2; ++part) {
-    const int32_t* pages = part == 0 ? p.prefix_pages : p.table + static_cast<int64_t>(r) * d.table_width;
-    const int count = part == 0 ? d.prefix_len : seen;
-    for (int j0 = 0; j0 < count; j0 += 32) {
-      const int j = j0 + lane;
-      int page = -1;
-      float s = -INFINITY;
-      if (j < count) {
-        page = __ldg(pages + (j >> p.page_shift));
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(d.num_pages)) page = -1;
-        s = 0.0f;
-        if (page >= 0) {
-          const uint16_t* k = p.kc + page * d.kc_page_stride + kvh * d.kc_head_stride +
-                              (j & (d.page_size - 1)) * d.kc_token_stride;
-          for (int e = 0; e < D; e += 8) {
-            const uint4 w = *reinterpret_cast<const uint4*>(k + e);
-            const uint16_t* x = reinterpret_cast<const uint16_t*>(&w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s = fmaf(s_q[warp][e + i], widen<BF16>(x[i]), s);
-          }
-        }
-        s *= p.scale_log2;
-      }
-      float top = s;
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float mn = fmaxf(m, top);
-      const float base = mn == -INFINITY ? 0.0f : mn;
-      const float keep = exp2f(m - base);
-      m = mn;
-      const float w = j < count ? exp2f(s - base) : 0.0f;
-      float sum = w;
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      l = l * keep + sum;
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] *= keep;
-      const int here = min(32, count - j0);
-      for (int i = 0; i < here; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, i);
-        const int pg = __shfl_sync(0xffffffffu, page, i);
-        if (pg < 0) continue;
-        const uint16_t* v = p.vc + pg * d.vc_page_stride + kvh * d.vc_head_stride +
-                            ((j0 + i) & (d.page_size - 1)) * d.vc_token_stride;
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wi, widen<BF16>(v[lane + 32 * e]), acc[e]);
-      }
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+  for (int i = 0; i < parts; ++i) {
+    const float2 ml = __ldcg(p.part_ml + i * rows + row);
+    if (ml.y == 0.0f) continue;  // nothing seen in that part
+    const float f = exp2_fast(ml.x - base);
+    l += ml.y * f;
+    const float* o = p.part_o + (i * rows + row) * D + lane * kPer;
+    if constexpr (kPer == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(o));
+      acc[0] += v.x * f;
+      acc[1] += v.y * f;
+      acc[2] += v.z * f;
+      acc[3] += v.w * f;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(o));
+      acc[0] += v.x * f;
+      acc[1] += v.y * f;
     }
   }
-  uint16_t* o = p.out + n * d.out_token_stride + h * d.out_head_stride;
-  const bool empty = m == -INFINITY;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = p.out + n * d.out_token_stride + h * d.out_head_stride + lane * kPer;
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) o[lane + 32 * e] = narrow<BF16>(empty ? 0.0f : acc[e] / l);
-  if (p.lse && lane == 0)
-    p.lse[static_cast<int64_t>(n) * d.heads + h] = empty ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack16<BF16>(acc[e] * inv, acc[e + 1] * inv);
+  if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+vqb_status launch_join(const AttnParams& p, int parts, bool bf, cudaStream_t s) {
+  const unsigned blocks = static_cast<unsigned>((part_rows(p.d) + 7) / 8);
+  cudaError_t ce;
+  if (p.d.head_dim == 128)
+    ce = bf ? launch_pdl(attention_join_kernel<128, true>, blocks, 256, 0, s, p, parts)
+            : launch_pdl(attention_join_kernel<128, false>, blocks, 256, 0, s, p, parts);
+  else
+    ce = bf ? launch_pdl(attention_join_kernel<64, true>, blocks, 256, 0, s, p, parts)
+            : launch_pdl(attention_join_kernel<64, false>, blocks, 256, 0, s, p, parts);
+  if (ce != cudaSuccess) return VQB_CUDA_ERROR;
+  note_launch();
+  return VQB_OK;
 }
 
 // Everything about a call that does not need its pointers.
 vqb_status check_desc(const vqb_attention_desc& d) {
   if (d.n_requests < 0 || d.n_tokens < 0 || d.heads < 1 || d.kv_heads < 1 || d.heads % d.kv_heads || d.max_q_len < 0 ||
-      d.max_kv_len < 0 || d.prefix_len < 0 || d.num_pages < 0 || d.table_width < 0)
+      d.max_kv_len < 0 || d.prefix_len < 0 || d.num_pages < 1 || d.table_width < 0)
     return VQB_BAD_SHAPE;
   if (!(d.scale > 0.0f) || d.scale > 3.0e38f) return VQB_BAD_SHAPE;
   if (d.head_dim != 64 && d.head_dim != 128) return VQB_UNSUPPORTED_GEOMETRY;
   if (d.page_size < 16 || d.page_size > 1024 || (d.page_size & (d.page_size - 1))) return VQB_UNSUPPORTED_GEOMETRY;
   if (d.heads > 65535 || d.n_requests > 65535) return VQB_UNSUPPORTED_GEOMETRY;
+  if (static_cast<int64_t>(d.n_tokens) * d.heads > 0x7fffffff) return VQB_UNSUPPORTED_GEOMETRY;
   if (static_cast<int64_t>(d.table_width) * d.page_size < d.max_kv_len) return VQB_BAD_SHAPE;
+  if (static_cast<int64_t>(d.prefix_len) + d.max_kv_len > 0x7fff0000) return VQB_UNSUPPORTED_GEOMETRY;
   const int64_t strides[] = {d.q_token_stride, d.q_head_stride, d.out_token_stride, d.out_head_stride,
                              d.kc_page_stride, d.kc_head_stride, d.kc_token_stride,
                              d.vc_page_stride, d.vc_head_stride, d.vc_token_stride};
@@ -148,6 +174,10 @@ vqb_status check_desc(const vqb_attention_desc& d) {
   return VQB_OK;
 }
 
+// SMs the plan counts on: the plan must not depend on the device that happens
+// to be current, so that the workspace's size fits the call.
+constexpr int kPlanSms = 148;
+
 }  // namespace
 }  // namespace vqb
 
@@ -155,7 +185,8 @@ using namespace vqb;
 
 extern "C" size_t vqb_prefix_attention_workspace_size(const vqb_attention_desc* desc) {
   if (!desc || check_desc(*desc) != VQB_OK) return 0;
-  return 256;
+  const AttnPlan a = make_plan(*desc, kPlanSms);
+  return kStatusBytes + ml_bytes(*desc, a.parts) + a.parts * part_rows(*desc) * desc->head_dim * sizeof(float);
 }
 
 extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_dtype dtype, const void* q,
@@ -165,7 +196,7 @@ extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_d
                                            vqb_stream_t stream) {
   if (!desc) return VQB_NULL_POINTER;
   const vqb_attention_desc& d = *desc;
-  const vqb_status st = check_desc(d);
+  vqb_status st = check_desc(d);
   if (st != VQB_OK) return st;
   if (dtype != VQB_F16 && dtype != VQB_BF16) return VQB_UNSUPPORTED_GEOMETRY;
   if (d.n_tokens == 0 || d.n_requests == 0) return VQB_OK;
@@ -175,24 +206,24 @@ extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_d
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return VQB_BAD_ALIGNMENT;
   if (workspace_bytes < vqb_prefix_attention_workspace_size(desc)) return VQB_WORKSPACE_TOO_SMALL;
+  const AttnPlan a = make_plan(d, kPlanSms);
+  const bool bf = dtype == VQB_BF16;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
   AttnParams p{d, static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache),
                static_cast<const uint16_t*>(v_cache), block_table, kv_lens, cu_q, prefix_pages,
-               static_cast<uint16_t*>(out), lse, d.heads / d.kv_heads, __builtin_ctz(d.page_size),
-               d.scale * 1.4426950408889634f};
-  const int64_t rows = static_cast<int64_t>(d.n_tokens) * d.heads;
-  if ((rows + 7) / 8 > 0x7fffffff) return VQB_UNSUPPORTED_GEOMETRY;
-  const unsigned blocks = static_cast<unsigned>((rows + 7) / 8);
+               static_cast<uint16_t*>(out), lse, reinterpret_cast<float*>(ws + kStatusBytes + ml_bytes(d, a.parts)),
+               reinterpret_cast<float2*>(ws + kStatusBytes), reinterpret_cast<int*>(ws) + 1, d.heads / d.kv_heads,
+               __builtin_ctz(d.page_size), d.scale * 1.4426950408889634f};
   if (cudaMemsetAsync(workspace, 0, 16, s) != cudaSuccess) return VQB_CUDA_ERROR;
-  cudaError_t ce;
-  const bool bf = dtype == VQB_BF16;
-  if (d.head_dim == 128)
-    ce = bf ? launch_pdl(attention_rows_kernel<true, 128>, blocks, 256, 0, s, p)
-            : launch_pdl(attention_rows_kernel<false, 128>, blocks, 256, 0, s, p);
-  else
-    ce = bf ? launch_pdl(attention_rows_kernel<true, 64>, blocks, 256, 0, s, p)
-            : launch_pdl(attention_rows_kernel<false, 64>, blocks, 256, 0, s, p);
-  if (ce != cudaSuccess) return VQB_CUDA_ERROR;
-  note_launch();
-  return VQB_OK;
+  timer_before(s);
+  if (a.shared.splits > 0) {
+    st = launch_attention_tiles(p, a.shared, bf, a.shared_tiles, s);
+    if (st != VQB_OK) return st;
+  }
+  st = a.decode ? launch_attention_decode(p, a.own, bf, s) : launch_attention_tiles(p, a.own, bf, a.own_tiles, s);
+  if (st != VQB_OK) return st;
+  if (a.parts > 0) st = launch_join(p, a.parts, bf, s);
+  timer_after(s);
+  return st;
 }

@@ -1,0 +1,314 @@
+// Attention of requests with few query rows (tokens x heads of a group <= 16)
+// over their own keys: one pass over the cache, bound by its bytes.
+//
+// A block takes (request, key/value head, a run of keys).  Its four warps are
+// independent: each streams every fourth group of 16 keys through its own ring
+// of shared-memory stages (four 2 KB TMA boxes a stage at D = 128; the warp's
+// first lane refills a stage as soon as the warp has read it), with its own
+// running maximum and sum.  A warp computes S = Q K^T and O += P V with
+// m16n8k16 MMAs: Q and O stay in registers, P goes from the accumulator's
+// layout straight into the next MMA's operand.  These MMAs run far below the
+// tensor cores' rate, but a group's 8 KB take 350 cycles of an SM's share of
+// memory bandwidth and 64 of its MMA pipe.  At the end the four warps' results
+// are joined in shared memory.
+#include "vq_attention.cuh"
+
+namespace vqb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kUnit = 16;  // keys of a stage
+template <int D>
+constexpr int kStages = D == 128 ? 3 : 6;  // 24 KB a warp, 96 KB a block, two blocks an SM
+template <int D>
+constexpr int kHalfBytes = kUnit * D * 2;  // K or V of a stage
+template <int D>
+constexpr size_t decode_smem() { return 1024 + size_t(kWarps) * kStages<D> * 2 * kHalfBytes<D>; }
+
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t s_full[kWarps][kStages<D>];
+  __shared__ float s_m[kWarps][16], s_l[kWarps][16];
+  __shared__ int s_abort;
+  constexpr int NS = kStages<D>;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const vqb_attention_desc& d = p.d;
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int w = 0; w < kWarps; ++w)
+      for (int i = 0; i < NS; ++i) mbar_init(&s_full[w][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  pdl_wait();
+
+  const int kvh = blockIdx.y, r = blockIdx.z, split = blockIdx.x;
+  const RequestRows rq = request_rows(p, r);
+  const int nrows = min(rq.nq * p.group, 16);
+  if (nrows == 0) return;
+  const int seg0 = pass.prefix ? d.prefix_len : 0;
+  const int seg1 = visible(p, rq, rq.nq - 1);
+  const int tiles0 = (seg0 + kUnit - 1) / kUnit, tiles = tiles0 + (seg1 + kUnit - 1) / kUnit;
+  const int per = pass.chunk / kUnit;
+  const int u0 = min(split * per, tiles), u1 = min(u0 + per, tiles);
+  // this warp's groups: u0 + warp, then every fourth
+  const int n = u1 - u0 > warp ? (u1 - u0 - warp + kWarps - 1) / kWarps : 0;
+  unsigned char* ring = smem + static_cast<size_t>(warp) * NS * 2 * kHalfBytes<D>;
+
+  auto page_of = [&](int k) -> int {  // page of the warp's k-th group
+    if (k >= n) return d.num_pages;
+    const int u = u0 + warp + kWarps * k;
+    const int page = u < tiles0 ? __ldg(p.prefix_pages + ((u * kUnit) >> p.page_shift))
+                                : __ldg(p.table + static_cast<int64_t>(r) * d.table_width +
+                                        (((u - tiles0) * kUnit) >> p.page_shift));
+    return static_cast<unsigned>(page) < static_cast<unsigned>(d.num_pages) ? page : d.num_pages;  // past the end: zeros
+  };
+  auto issue = [&](int k, int page) {  // one lane
+    const int u = u0 + warp + kWarps * k;
+    const int key = (u < tiles0 ? u : u - tiles0) * kUnit;
+    const int off = key & (d.page_size - 1);
+    uint64_t* bar = &s_full[warp][k % NS];
+    unsigned char* dst = ring + (k % NS) * 2 * kHalfBytes<D>;
+    mbar_expect_tx(bar, 2 * kHalfBytes<D>);
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) tma_load_4d(&kmap, bar, dst + h * 2048, h * 64, off, kvh, page);
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) tma_load_4d(&vmap, bar, dst + kHalfBytes<D> + h * 2048, h * 64, off, kvh, page);
+  };
+
+  // pages of 32 groups at a time, one a lane; the next 32 are fetched while these are used
+  int pages = page_of(lane), pages_next = page_of(32 + lane);
+  for (int k = 0; k < NS; ++k) {
+    const int pg = __shfl_sync(0xffffffffu, pages, k);
+    if (k < n && lane == 0) issue(k, pg);
+  }
+
+  // Q as the first operand: rows lane / 4 and lane / 4 + 8
+  const int row0 = lane >> 2, row1 = row0 + 8;
+  uint32_t qf[D / 16][4];
+  {
+    auto qrow = [&](int row) {
+      return p.q + (rq.q0 + row / p.group) * d.q_token_stride + (kvh * p.group + row % p.group) * d.q_head_stride;
+    };
+    const uint16_t* a = qrow(row0 < nrows ? row0 : 0);
+    const uint16_t* b = qrow(row1 < nrows ? row1 : 0);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int e = ks * 16 + (lane & 3) * 2;
+      qf[ks][0] = row0 < nrows ? *reinterpret_cast<const uint32_t*>(a + e) : 0u;
+      qf[ks][1] = row1 < nrows ? *reinterpret_cast<const uint32_t*>(b + e) : 0u;
+      qf[ks][2] = row0 < nrows ? *reinterpret_cast<const uint32_t*>(a + e + 8) : 0u;
+      qf[ks][3] = row1 < nrows ? *reinterpret_cast<const uint32_t*>(b + e + 8) : 0u;
+    }
+  }
+  const int vis0 = visible(p, rq, min(row0 / p.group, rq.nq - 1)), vis1 = visible(p, rq, min(row1 / p.group, rq.nq - 1));
+  pdl_trigger();
+
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+  // a lane's row address for the two kinds of 8x8 matrix loads
+  const int krow = ((lane >> 4) << 3) + (lane & 7), kchunk = (lane >> 3) & 1;
+  const int vrow = (((lane >> 3) & 1) << 3) + (lane & 7), vchunk = lane >> 4;
+  for (int k = 0; k < n; ++k) {
+    if (!warp_wait(&s_full[warp][k % NS], (k / NS) & 1, &s_abort)) {
+      // gave up: copies in flight must land before the ring is used again
+      for (int j = k; lane == 0 && j < min(k + NS, n); ++j) mbar_drain(&s_full[warp][j % NS], (j / NS) & 1);
+      if (lane == 0) *p.status = VQB_TIMEOUT;
+      break;
+    }
+    const int u = u0 + warp + kWarps * k;
+    const bool own = u >= tiles0;
+    const int key = (own ? u - tiles0 : u) * kUnit;
+    const uint32_t kb = smem_u32(ring + (k % NS) * 2 * kHalfBytes<D>), vb = kb + kHalfBytes<D>;
+    const int lim0 = min((own ? vis0 : seg0) - key, kUnit), lim1 = min((own ? vis1 : seg0) - key, kUnit);
+    const int held = min((own ? seg1 : seg0) - key, kUnit);
+    if (held < kUnit) {
+      // what lies past the last key may be anything: its weight is 0, its value must be finite
+      unsigned char* v = ring + (k % NS) * 2 * kHalfBytes<D> + kHalfBytes<D>;
+      for (int i = lane; i < (kUnit - held) * (D / 8); i += 32) {
+        const int rr = held + i / (D / 8), c = i % (D / 8);
+        *reinterpret_cast<uint4*>(v + (c >> 3) * 2048 + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a copy reuses the stage
+      __syncwarp();
+    }
+    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t b[4];
+      const int c = ks * 2 + kchunk;
+      ldsm4(b, kb + (c >> 3) * 2048 + krow * 128 + (((c & 7) ^ (krow & 7)) << 4));
+      mma16816<BF16>(s[0], qf[ks], b[0], b[1]);
+      mma16816<BF16>(s[1], qf[ks], b[2], b[3]);
+    }
+    if (__any_sync(0xffffffffu, lim0 < kUnit || lim1 < kUnit)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = t * 8 + (lane & 3) * 2 + e;
+          if (col >= lim0) s[t][e] = -INFINITY;
+          if (col >= lim1) s[t][2 + e] = -INFINITY;
+        }
+    }
+    float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+    float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+    t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
+    t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
+    t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)) * p.scale_log2;
+    t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2)) * p.scale_log2;
+    if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack)) {
+      const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+      const float f0 = n0 == -INFINITY ? 1.0f : exp2_fast(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : exp2_fast(m1 - n1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= f0;
+      l1 *= f1;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= f0;
+        o[i][1] *= f0;
+        o[i][2] *= f1;
+        o[i][3] *= f1;
+      }
+    }
+    const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t][0] = exp2_fast(fmaf(s[t][0], p.scale_log2, -b0));
+      s[t][1] = exp2_fast(fmaf(s[t][1], p.scale_log2, -b0));
+      s[t][2] = exp2_fast(fmaf(s[t][2], p.scale_log2, -b1));
+      s[t][3] = exp2_fast(fmaf(s[t][3], p.scale_log2, -b1));
+      l0 += s[t][0] + s[t][1];
+      l1 += s[t][2] + s[t][3];
+    }
+    const uint32_t pf[4] = {pack16<BF16>(s[0][0], s[0][1]), pack16<BF16>(s[0][2], s[0][3]),
+                            pack16<BF16>(s[1][0], s[1][1]), pack16<BF16>(s[1][2], s[1][3])};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t b[4];
+      const int c = i * 2 + vchunk;
+      ldsm4_t(b, vb + (c >> 3) * 2048 + vrow * 128 + (((c & 7) ^ (vrow & 7)) << 4));
+      mma16816<BF16>(o[2 * i], pf, b[0], b[1]);
+      mma16816<BF16>(o[2 * i + 1], pf, b[2], b[3]);
+    }
+    __syncwarp();
+    const int next = k + NS;
+    if ((next & 31) == 0) {
+      pages = pages_next;
+      pages_next = page_of(next + 32 + lane);
+    }
+    const int pg = __shfl_sync(0xffffffffu, pages, next & 31);
+    if (next < n && lane == 0) issue(next, pg);
+  }
+  l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+  l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+  l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+  l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+  __syncwarp();
+
+  // ---- the four warps' results, joined: each leaves its own in its ring
+  float* mine = reinterpret_cast<float*>(ring);  // [16][D]
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    const int e = i * 8 + (lane & 3) * 2;
+    *reinterpret_cast<float2*>(mine + row0 * D + e) = make_float2(o[i][0], o[i][1]);
+    *reinterpret_cast<float2*>(mine + row1 * D + e) = make_float2(o[i][2], o[i][3]);
+  }
+  if ((lane & 3) == 0) {
+    s_m[warp][row0] = m0;
+    s_l[warp][row0] = l0;
+    s_m[warp][row1] = m1;
+    s_l[warp][row1] = l1;
+  }
+  __syncthreads();
+  constexpr int kPer = D / 4;  // threads of a row, four elements each
+  constexpr size_t kRing = size_t(NS) * 2 * kHalfBytes<D> / sizeof(float);
+  const float* rings = reinterpret_cast<const float*>(smem);
+  for (int i = threadIdx.x; i < nrows * kPer; i += kWarps * 32) {
+    const int row = i / kPer, e = (i % kPer) * 4;
+    float m = s_m[0][row];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w][row]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2_fast(s_m[w][row] - base);
+      const float4 x = *reinterpret_cast<const float4*>(rings + w * kRing + row * D + e);
+      l += s_l[w][row] * f;
+      a.x += x.x * f;
+      a.y += x.y * f;
+      a.z += x.z * f;
+      a.w += x.w * f;
+    }
+    const int64_t tok = rq.q0 + row / p.group;
+    const int head = kvh * p.group + row % p.group;
+    const int64_t grow = tok * d.heads + head;
+    if (pass.part0 >= 0) {
+      const int64_t at = (pass.part0 + split) * (static_cast<int64_t>(d.n_tokens) * d.heads) + grow;
+      *reinterpret_cast<float4*>(p.part_o + at * D + e) = a;
+      if (e == 0) p.part_ml[at] = make_float2(m, l);
+    } else {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const uint2 w = make_uint2(pack16<BF16>(a.x * inv, a.y * inv), pack16<BF16>(a.z * inv, a.w * inv));
+      *reinterpret_cast<uint2*>(p.out + tok * d.out_token_stride + head * d.out_head_stride + e) = w;
+      if (p.lse && e == 0) p.lse[grow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    }
+  }
+}
+
+template <int D, bool BF16>
+vqb_status launch(const AttnParams& p, const AttnPass& pass, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  constexpr size_t smem = decode_smem<D>();
+  if (cudaFuncSetAttribute(attention_decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem)) != cudaSuccess)
+    return VQB_CUDA_ERROR;
+  const dim3 grid(pass.splits, p.d.kv_heads, p.d.n_requests);
+  if (launch_pdl(attention_decode_kernel<D, BF16>, grid, kWarps * 32, smem, s, p, pass, km, vm) != cudaSuccess)
+    return VQB_CUDA_ERROR;
+  note_launch();
+  return VQB_OK;
+}
+
+}  // namespace
+
+vqb_status launch_attention_decode(const AttnParams& p, const AttnPass& pass, bool bf16, cudaStream_t s) {
+  CUtensorMap km, vm;
+  const vqb_attention_desc& d = p.d;
+  vqb_status st = encode_pool(&km, d, bf16, p.kc, d.kc_page_stride, d.kc_head_stride, d.kc_token_stride, kUnit);
+  if (st != VQB_OK) return st;
+  st = encode_pool(&vm, d, bf16, p.vc, d.vc_page_stride, d.vc_head_stride, d.vc_token_stride, kUnit);
+  if (st != VQB_OK) return st;
+  if (d.head_dim == 128) return bf16 ? launch<128, true>(p, pass, km, vm, s) : launch<128, false>(p, pass, km, vm, s);
+  return bf16 ? launch<64, true>(p, pass, km, vm, s) : launch<64, false>(p, pass, km, vm, s);
+}
+
+}  // namespace vqb

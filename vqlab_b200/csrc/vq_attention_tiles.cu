@@ -1,0 +1,483 @@
+// Attention of many query rows over common keys on the 5th-generation tensor
+// cores: a long prompt over its own cache, or the rows of a whole batch over the
+// prefix that it shares (each prefix page is then read once for 256 rows
+// instead of once a request).
+//
+// A block takes (256 rows of one key/value head, a run of keys): two tiles of
+// 128 rows (a row = a token and a head of the group) that share every K and V
+// tile of 128 keys.  Roles:
+//   * a TMA warp fills a ring of shared-memory stages with K and V tiles, one
+//     box a page and 64 elements (a lane a page);
+//   * one thread issues the MMAs: S_t = Q_t K^T (both from shared memory) into
+//     tensor memory, then O_t += P_t V with P_t in tensor memory over S_t's
+//     columns and V read along its other dimension.  Order: P0 V, Q0 K'^T, P1 V,
+//     Q1 K'^T: while one tile's softmax runs, the other's products do;
+//   * four softmax warps a tile, a thread a row: the row's 128 scores into
+//     registers, running maximum and sum, weights as 16-bit numbers back to
+//     tensor memory.  O is rescaled in place, by the same thread, only when the
+//     maximum has grown by more than 2^kSlack.
+// Scores, weights' sum and O are fp32; the weights are rounded once to the
+// cache's type, which the MMA needs.
+//
+// Every wait is bounded (2 s): on expiry the block records VQB_TIMEOUT, waits for
+// its copies and MMAs in flight, frees its tensor memory and returns.
+#include "vq_attention.cuh"
+
+namespace vqb {
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kTileKeys = 128;
+constexpr int kThreads = 320;
+constexpr int kWarpMma = 8, kWarpTma = 9;
+constexpr int kTmemCols = 512;
+template <int D>
+constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
+template <int D>
+constexpr int kStages = D == 128 ? 5 : 8;
+template <int D>
+constexpr size_t tiles_smem() {
+  return 1024 + size_t(2) * kTileRows * D * 2 + size_t(kStages<D>) * kStageBytes<D> + 256;
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+               :: "r"(smem_u32(bar)) : "memory");
+}
+// D (+)= A B, A and B in shared memory
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+}
+// D (+)= A B, A in tensor memory
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+}
+#define VQB_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define VQB_S8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : VQB_R8(v, 0), VQB_R8(v, 8), VQB_R8(v, 16), VQB_R8(v, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      :: "r"(addr), VQB_S8(v, 0), VQB_S8(v, 8), VQB_S8(v, 16), VQB_S8(v, 24) : "memory");
+}
+
+// Shared-memory matrix descriptors, 128-byte swizzle: start >> 4 at [0,14),
+// leading byte offset >> 4 at [16,30), stride byte offset >> 4 at [32,46),
+// version 1 at [46,48), layout type 2 at [61,64).  Q and K: the contracted
+// dimension is contiguous, 8-row groups 1024 bytes apart.  V: the output
+// dimension is contiguous, 64 elements a row; 8-key groups 1024 bytes apart
+// (stride), the second 64 elements a whole half tile away (leading).
+__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t leading) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(leading >> 4) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) | (static_cast<uint64_t>(2u) << 61);
+}
+// kind::f16, fp32 accumulator, A and B of one 16-bit type, N >> 3 at [17,23),
+// M >> 4 at [24,29); bit 16: B's output dimension is the contiguous one.
+template <bool BF16>
+__device__ __forceinline__ constexpr uint32_t idesc_f16(int n, bool b_along_n) {
+  return (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((b_along_n ? 1u : 0u) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileRows >> 4) << 24);
+}
+
+// What a block works on.
+struct TileWork {
+  RequestRows rq;
+  int request;
+  int row0, rows;  // its first row, and rows of the request (tokens x group)
+  int seg0, seg1;  // keys: of the prefix, of the request itself
+};
+
+// The block's request and rows.  joint: all tokens are one run of rows.  Else
+// blocks count pairs of tiles over the requests, the last first (a causal
+// prompt's last tiles have the most keys).  false: nothing there.
+__device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& pass, int block, int lane, TileWork* w) {
+  constexpr int kRows = 2 * kTileRows;
+  const vqb_attention_desc& d = p.d;
+  if (pass.joint) {
+    w->request = -1;
+    w->rq.q0 = 0;
+    w->rq.nq = min(__ldg(p.cu_q + d.n_requests), d.n_tokens);
+    w->rq.len = 0;
+    w->row0 = block * kRows;
+    w->rows = w->rq.nq * p.group;
+    w->seg0 = d.prefix_len;
+    w->seg1 = 0;
+    return w->row0 < w->rows;
+  }
+  int before = 0;
+  for (int base = d.n_requests; base > 0; base -= 32) {
+    const int r = base - 1 - lane;
+    RequestRows rq{0, 0, 0};
+    if (r >= 0) rq = request_rows(p, r);
+    const int pairs = (min(rq.nq, d.max_q_len) * p.group + kRows - 1) / kRows;
+    int inc = pairs;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > block);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int first = before + __shfl_sync(0xffffffffu, inc - pairs, src);
+      const int np = __shfl_sync(0xffffffffu, pairs, src);
+      w->request = base - 1 - src;
+      w->rq.q0 = __shfl_sync(0xffffffffu, rq.q0, src);
+      w->rq.nq = __shfl_sync(0xffffffffu, rq.nq, src);
+      w->rq.len = __shfl_sync(0xffffffffu, rq.len, src);
+      w->rows = min(w->rq.nq, d.max_q_len) * p.group;
+      w->row0 = (np - 1 - (block - first)) * kRows;
+      w->seg0 = pass.prefix ? d.prefix_len : 0;
+      const int last = min(w->row0 + kRows, w->rows) - 1;
+      w->seg1 = visible(p, w->rq, last / p.group);
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return false;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+  extern __shared__ unsigned char smem_raw[];
+  constexpr int NS = kStages<D>;
+  constexpr int kHalf = kTileKeys * 128;  // 64 elements of 128 rows
+  constexpr int kQTile = kTileRows * D * 2;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* q_s = smem;
+  unsigned char* ring = smem + 2 * kQTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * kStageBytes<D>);
+  uint64_t* kv_full = bars;            // [NS] the stage's copies landed
+  uint64_t* kv_empty = bars + NS;      // [NS] the MMAs that read the stage are done
+  uint64_t* s_full = kv_empty + NS;    // [2] a tile's scores are in tensor memory
+  uint64_t* p_full = s_full + 2;       // [2] its weights are (four warps)
+  uint64_t* o_full = p_full + 2;       // [2] its O has this key tile
+  uint64_t* mma_done = o_full + 2;     // [1] teardown
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const vqb_attention_desc& d = p.d;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+  TileWork w;
+  if (!find_work(p, pass, blockIdx.x, lane, &w)) return;  // the same for every thread
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  const int tiles0 = (w.seg0 + kTileKeys - 1) / kTileKeys, all = tiles0 + (w.seg1 + kTileKeys - 1) / kTileKeys;
+  const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / pass.splits);
+  const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / pass.splits) - t0;
+  const int active = w.rows - w.row0 > kTileRows ? 2 : 1;
+
+  // ---- Q into shared memory (128-byte swizzle), rows past the last as zeros
+  for (int i = threadIdx.x; i < active * kTileRows * (D / 8); i += kThreads) {
+    const int row = i / (D / 8), c = i % (D / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    const int g = w.row0 + row;
+    if (g < w.rows) {
+      const int tok = g / p.group;
+      v = *reinterpret_cast<const uint4*>(p.q + (w.rq.q0 + tok) * d.q_token_stride +
+                                          (kvh * p.group + (g - tok * p.group)) * d.q_head_stride + c * 8);
+    }
+    const int tr = row & (kTileRows - 1);
+    *reinterpret_cast<uint4*>(q_s + (row / kTileRows) * kQTile + (c >> 3) * kHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = v;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // the columns of tile t's scores (its weights lie over them) and output
+  auto s_col = [&](int t) { return tmem + t * kTileKeys; };
+  auto o_col = [&](int t) { return tmem + 2 * kTileKeys + t * D; };
+
+  if (warp == kWarpTma) {
+    // ---------------- K and V tiles: a lane loads a page
+    const int box = min(d.page_size, kTileKeys);
+    auto page_of = [&](int i) -> int {  // the lane's page of the i-th tile (past the pool: read as zeros)
+      if (i >= n) return d.num_pages;
+      const bool own = t0 + i >= tiles0;
+      const int start = (own ? t0 + i - tiles0 : t0 + i) * kTileKeys, key = start + lane * box;
+      if (lane * box >= kTileKeys || key >= (own ? w.seg1 : w.seg0)) return d.num_pages;
+      const int page = own ? __ldg(p.table + static_cast<int64_t>(w.request) * d.table_width + (key >> p.page_shift))
+                           : __ldg(p.prefix_pages + (key >> p.page_shift));
+      return static_cast<unsigned>(page) < static_cast<unsigned>(d.num_pages) ? page : d.num_pages;
+    };
+    int page = page_of(0);
+    bool ok = true;
+    int issued = 0;
+    for (int i = 0; i < n && ok; ++i) {
+      const int page_next = page_of(i + 1);
+      const bool own = t0 + i >= tiles0;
+      const int start = (own ? t0 + i - tiles0 : t0 + i) * kTileKeys;
+      const int held = min((own ? w.seg1 : w.seg0) - start, kTileKeys);
+      const int boxes = (held + box - 1) / box;
+#pragma unroll
+      for (int kv = 0; kv < 2 && ok; ++kv) {
+        const int st = (2 * i + kv) % NS;
+        if (!warp_wait(&kv_empty[st], (((2 * i + kv) / NS) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(&kv_full[st], static_cast<uint32_t>(boxes * box * D * 2));
+        __syncwarp();
+        ++issued;
+        if (lane < boxes) {
+          unsigned char* dst = ring + st * kStageBytes<D> + lane * box * 128;
+          const int off = (start + lane * box) & (d.page_size - 1);
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_4d(kv == 0 ? &kmap : &vmap, &kv_full[st], dst + h * kHalf, h * 64, off, kvh, page);
+        }
+      }
+      page = page_next;
+    }
+    // no copy may still be writing shared memory when the block ends
+    if (lane == 0)
+      for (int k = max(issued - NS, 0); k < issued; ++k) mbar_drain(&kv_full[k % NS], (k / NS) & 1);
+  } else if (warp == kWarpMma) {
+    // ---------------- the MMAs, one thread
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t qk = idesc_f16<BF16>(kTileKeys, false), pv = idesc_f16<BF16>(D, true);
+      auto stage = [&](int idx) { return smem_u32(ring + (idx % NS) * kStageBytes<D>); };
+      auto wait_kv = [&](int idx) { return mbar_wait(&kv_full[idx % NS], (idx / NS) & 1, abort_flag); };
+      auto mma_qk = [&](int t, int i) {
+        const uint32_t qa = smem_u32(q_s + t * kQTile), kb = stage(2 * i);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
+          tc_mma_ss(s_col(t), desc128(qa + off, 16), desc128(kb + off, 16), qk, ks > 0);
+        }
+        tc_commit(&s_full[t]);
+      };
+      auto held_of = [&](int i) {
+        const bool own = t0 + i >= tiles0;
+        return min((own ? w.seg1 : w.seg0) - (own ? t0 + i - tiles0 : t0 + i) * kTileKeys, kTileKeys);
+      };
+      bool ok = wait_kv(0);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < active; ++t) mma_qk(t, 0);
+        tc_commit(&kv_empty[0]);
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        const int steps = (held_of(i) + 15) / 16;
+        for (int t = 0; t < active && ok; ++t) {
+          ok = mbar_wait(&p_full[t], i & 1, abort_flag) && (t > 0 || wait_kv(2 * i + 1));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t vb = stage(2 * i + 1);
+          for (int ks = 0; ks < steps; ++ks)
+            tc_mma_ts(o_col(t), s_col(t) + ks * 8, desc128(vb + ks * 2048, kHalf), pv, i > 0 || ks > 0);
+          tc_commit(&o_full[t]);
+          if (i + 1 < n) {
+            if (t == 0) {
+              ok = wait_kv(2 * i + 2);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            mma_qk(t, i + 1);
+          }
+        }
+        if (!ok) break;
+        tc_commit(&kv_empty[(2 * i + 1) % NS]);
+        if (i + 1 < n) tc_commit(&kv_empty[(2 * i + 2) % NS]);
+      }
+      tc_commit(mma_done);
+      mbar_drain(mma_done, 0);
+    }
+  } else {
+    // ---------------- softmax: a thread a row
+    const int t = warp >> 2;
+    if (t < active) {
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const int g = w.row0 + t * kTileRows + (warp & 3) * 32 + lane;
+      const int gv = min(g, w.rows - 1), tok = gv / p.group;
+      const int vis = pass.joint ? 0 : visible(p, w.rq, tok);
+      float m = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int i = 0; i < n; ++i) {
+        const bool own = t0 + i >= tiles0;
+        const int start = (own ? t0 + i - tiles0 : t0 + i) * kTileKeys;
+        const int held = min((own ? w.seg1 : w.seg0) - start, kTileKeys);
+        const int lim = own ? vis - start : held;
+        if (!(ok = warp_wait(&s_full[t], i & 1, abort_flag))) break;
+        // the MMAs of the key tile before this one came first: done already, waited for to keep in step with the barrier
+        if (i > 0 && !(ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc_ld32(s_col(t) + lanes + c * 32, s + c * 32);
+        tc_wait_ld();
+        if (__any_sync(0xffffffffu, lim < kTileKeys)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= lim) s[c] = 0xFF800000u;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(s[c]));
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+        if (__any_sync(0xffffffffu, mx > m + kSlack)) {
+          const float mn = fmaxf(m, mx);
+          const float f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
+          m = mn;
+          l *= f;
+          if (i > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tc_ld32(o_col(t) + lanes + c * 32, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc_st32(o_col(t) + lanes + c * 32, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float a = exp2_fast(fmaf(__uint_as_float(s[h * 64 + 2 * c]), p.scale_log2, -base));
+            const float b = exp2_fast(fmaf(__uint_as_float(s[h * 64 + 2 * c + 1]), p.scale_log2, -base));
+            sum[(2 * c) & 3] += a;
+            sum[(2 * c + 1) & 3] += b;
+            pk[c] = pack16<BF16>(a, b);
+          }
+          tc_st32(s_col(t) + lanes + h * 32, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (t == 0 && (warp & 3) == 0 && (held & 15)) {
+          // what lies past the last key may be anything: its weight is 0, its value must be finite
+          const int st = (2 * i + 1) % NS;
+          if (!(ok = warp_wait(&kv_full[st], ((2 * i + 1) / NS) & 1, abort_flag))) break;
+          const int first = held, rows = ((held + 15) & ~15) - held;
+          for (int e = lane; e < rows * (D / 8); e += 32) {
+            const int rr = first + e / (D / 8), c = e % (D / 8);
+            *reinterpret_cast<uint4*>(ring + st * kStageBytes<D> + (c >> 3) * kHalf + rr * 128 + (c & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (ok && n > 0) ok = warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
+      if (!ok && lane == 0) *p.status = VQB_TIMEOUT;
+      if (ok) {
+        tc_fence_after();
+        const int64_t token = w.rq.q0 + tok;
+        const int head = kvh * p.group + (gv - tok * p.group);
+        const int64_t grow = token * d.heads + head;
+        const bool live = g < w.rows;
+        const bool partial = pass.part0 >= 0;
+        const int64_t at = (pass.part0 + split) * (static_cast<int64_t>(d.n_tokens) * d.heads) + grow;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (n > 0) {
+            tc_ld32(o_col(t) + lanes + c * 32, o);
+            tc_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          if (live && partial) {
+            uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + c * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else if (live) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              pk[e] = pack16<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            uint4* dst = reinterpret_cast<uint4*>(p.out + token * d.out_token_stride + head * d.out_head_stride + c * 32);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+          }
+          __syncwarp();
+        }
+        if (live) {
+          if (partial) p.part_ml[at] = make_float2(m, l);
+          else if (p.lse) p.lse[grow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <int D, bool BF16>
+vqb_status launch(const AttnParams& p, const AttnPass& pass, unsigned tiles, const CUtensorMap& km, const CUtensorMap& vm,
+                  cudaStream_t s) {
+  constexpr size_t smem = tiles_smem<D>();
+  static_assert(smem <= 232448, "over the opt-in shared memory of an SM");
+  if (cudaFuncSetAttribute(attention_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem)) != cudaSuccess)
+    return VQB_CUDA_ERROR;
+  const dim3 grid(tiles, p.d.kv_heads, pass.splits);
+  if (launch_pdl(attention_tiles_kernel<D, BF16>, grid, kThreads, smem, s, p, pass, km, vm) != cudaSuccess)
+    return VQB_CUDA_ERROR;
+  note_launch();
+  return VQB_OK;
+}
+
+}  // namespace
+
+// tiles: an upper bound of the pairs of row tiles of the pass.
+vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, unsigned tiles, cudaStream_t s) {
+  CUtensorMap km, vm;
+  const vqb_attention_desc& d = p.d;
+  const int box = d.page_size < kTileKeys ? d.page_size : kTileKeys;
+  vqb_status st = encode_pool(&km, d, bf16, p.kc, d.kc_page_stride, d.kc_head_stride, d.kc_token_stride, box);
+  if (st != VQB_OK) return st;
+  st = encode_pool(&vm, d, bf16, p.vc, d.vc_page_stride, d.vc_head_stride, d.vc_token_stride, box);
+  if (st != VQB_OK) return st;
+  if (d.head_dim == 128)
+    return bf16 ? launch<128, true>(p, pass, tiles, km, vm, s) : launch<128, false>(p, pass, tiles, km, vm, s);
+  return bf16 ? launch<64, true>(p, pass, tiles, km, vm, s) : launch<64, false>(p, pass, tiles, km, vm, s);
+}
+
+}  // namespace vqb
