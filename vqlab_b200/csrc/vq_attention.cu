@@ -57,7 +57,7 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   if (joint) {
     a.shared_tiles = static_cast<unsigned>(ceil_div(rows, 256));
     a.shared = AttnPass{1, 0, pick_splits(static_cast<int64_t>(a.shared_tiles) * d.kv_heads, ceil_div(d.prefix_len, 128),
-                                          sms, row_cost, true), 0, 0};
+                                          sms, row_cost, true), 0, 0, 1};
   }
   const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
   a.own.prefix = !joint && d.prefix_len > 0;
@@ -77,6 +77,7 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
     const int64_t blocks = (rows / 256 > d.n_requests ? rows / 256 : d.n_requests) * d.kv_heads;
     a.own.splits = pick_splits(blocks, ceil_div(keys, 128), sms, row_cost, joint);
   }
+  a.own.first = a.shared.splits == 0;
   a.parts = a.shared.splits + a.own.splits;
   a.own.part0 = a.shared.splits;
   if (a.parts == 1) {
@@ -215,7 +216,6 @@ extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_d
                static_cast<uint16_t*>(out), lse, reinterpret_cast<float*>(ws + kStatusBytes + ml_bytes(d, a.parts)),
                reinterpret_cast<float2*>(ws + kStatusBytes), reinterpret_cast<int*>(ws) + 1, d.heads / d.kv_heads,
                __builtin_ctz(d.page_size), d.scale * 1.4426950408889634f};
-  if (cudaMemsetAsync(workspace, 0, 16, s) != cudaSuccess) return VQB_CUDA_ERROR;
   timer_before(s);
   if (a.shared.splits > 0) {
     st = launch_attention_tiles(p, a.shared, bf, a.shared_tiles, s);

@@ -23,7 +23,7 @@ struct AttnParams {
   float* lse;
   float* part_o;
   float2* part_ml;
-  int* status;
+  int* status;      // int32 [1] of the workspace
   int group;
   int page_shift;
   float scale_log2;  // scale * log2(e): scores in powers of two
@@ -36,6 +36,7 @@ struct AttnPass {
   int splits;
   int part0;     // first partial result of the pass; -1: the pass writes out itself
   int chunk;     // decode kernel: keys of a split
+  int first;     // the call's first pass: its first block clears the status block
 };
 
 vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, unsigned tiles, cudaStream_t s);
@@ -64,6 +65,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// The status block starts at zero: written by the call's first block as it starts,
+// 2 s before any wait can give up.
+__device__ __forceinline__ void clear_status(const AttnParams& p, const AttnPass& pass) {
+  if (pass.first && (blockIdx.x | blockIdx.y | blockIdx.z) == 0 && threadIdx.x < 4) p.status[static_cast<int>(threadIdx.x) - 1] = 0;
 }
 
 // The queries of request r, as far as the call's bounds go.

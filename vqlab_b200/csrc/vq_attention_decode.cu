@@ -65,6 +65,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUt
   }
   __syncthreads();
   pdl_wait();
+  clear_status(p, pass);
 
   const int kvh = blockIdx.y, r = blockIdx.z, split = blockIdx.x;
   const RequestRows rq = request_rows(p, r);

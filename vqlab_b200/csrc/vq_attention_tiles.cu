@@ -63,6 +63,7 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
 }
 #define VQB_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define VQB_RW8(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7])
 #define VQB_S8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
 __device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* v) {
   asm volatile(
@@ -70,11 +71,101 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* v) {
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : VQB_R8(v, 0), VQB_R8(v, 8), VQB_R8(v, 16), VQB_R8(v, 24) : "r"(addr) : "memory");
 }
+// wait for the loads, and keep what uses these registers behind the wait
+__device__ __forceinline__ void tc_wait_ld32(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : VQB_RW8(v, 0), VQB_RW8(v, 8), VQB_RW8(v, 16), VQB_RW8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :: "r"(addr), VQB_S8(v, 0), VQB_S8(v, 8) : "memory");
+}
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
       :: "r"(addr), VQB_S8(v, 0), VQB_S8(v, 8), VQB_S8(v, 16), VQB_S8(v, 24) : "memory");
+}
+
+// pairs of fp32 numbers
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The scores of a row's 128 keys at tensor-memory address `addr`, 32 at a time,
+// the next 32 on their way while `use(chunk, scores)` works on these.  MASK:
+// scores from `lim` on become -inf.
+template <bool MASK, typename F>
+__device__ __forceinline__ void for_scores(uint32_t addr, int lim, F use) {
+  uint32_t a[32], b[32];
+  tc_ld32(addr, a);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t* v = (c & 1) ? b : a;
+    tc_wait_ld32(v);
+    if (c < 3) tc_ld32(addr + (c + 1) * 32, (c & 1) ? a : b);
+    if constexpr (MASK) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (c * 32 + e >= lim) v[e] = 0xFF800000u;
+    }
+    use(c, reinterpret_cast<const float*>(v));
+  }
+}
+template <bool MASK>
+__device__ __forceinline__ float scores_max(uint32_t addr, int lim) {
+  float t0 = -INFINITY, t1 = -INFINITY;
+  for_scores<MASK>(addr, lim, [&](int, const float* s) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      t0 = max3(t0, s[e], s[e + 1]);
+      t1 = max3(t1, s[e + 2], s[e + 3]);
+    }
+  });
+  return fmaxf(t0, t1);
+}
+// Weights 2^(score * scale - base) of the row's keys: to `addr` as 16-bit numbers,
+// over scores already read; returns their sum.
+template <bool MASK, bool BF16>
+__device__ __forceinline__ float scores_weights(uint32_t addr, int lim, float scale, float base) {
+  const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+  uint64_t sum0 = pair(0.f, 0.f), sum1 = sum0;
+  for_scores<MASK>(addr, lim, [&](int c, const float* s) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float2 x = unpair(fma2(pair(s[2 * e], s[2 * e + 1]), scale2, base2));
+      const float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+      if (e & 1) sum1 = add2(sum1, pair(w.x, w.y));
+      else sum0 = add2(sum0, pair(w.x, w.y));
+      pk[e] = pack16<BF16>(w.x, w.y);
+    }
+    tc_st16(addr + c * 16, pk);
+  });
+  const float2 t = unpair(add2(sum0, sum1));
+  return t.x + t.y;
 }
 
 // Shared-memory matrix descriptors, 128-byte swizzle: start >> 4 at [0,14),
@@ -190,6 +281,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_wait();
+  clear_status(p, pass);
   pdl_trigger();
   TileWork w;
   if (!find_work(p, pass, blockIdx.x, lane, &w)) return;  // the same for every thread
@@ -337,19 +429,9 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         // the MMAs of the key tile before this one came first: done already, waited for to keep in step with the barrier
         if (i > 0 && !(ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag))) break;
         tc_fence_after();
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tc_ld32(s_col(t) + lanes + c * 32, s + c * 32);
-        tc_wait_ld();
-        if (__any_sync(0xffffffffu, lim < kTileKeys)) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= lim) s[c] = 0xFF800000u;
-        }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(s[c]));
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+        const uint32_t srow = s_col(t) + lanes;
+        const bool mask = __any_sync(0xffffffffu, lim < kTileKeys);
+        const float mx = (mask ? scores_max<true>(srow, lim) : scores_max<false>(srow, lim)) * p.scale_log2;
         if (__any_sync(0xffffffffu, mx > m + kSlack)) {
           const float mn = fmaxf(m, mx);
           const float f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
@@ -368,21 +450,8 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
           }
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const float a = exp2_fast(fmaf(__uint_as_float(s[h * 64 + 2 * c]), p.scale_log2, -base));
-            const float b = exp2_fast(fmaf(__uint_as_float(s[h * 64 + 2 * c + 1]), p.scale_log2, -base));
-            sum[(2 * c) & 3] += a;
-            sum[(2 * c + 1) & 3] += b;
-            pk[c] = pack16<BF16>(a, b);
-          }
-          tc_st32(s_col(t) + lanes + h * 32, pk);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += mask ? scores_weights<true, BF16>(srow, lim, p.scale_log2, base)
+                  : scores_weights<false, BF16>(srow, lim, p.scale_log2, base);
         if (t == 0 && (warp & 3) == 0 && (held & 15)) {
           // what lies past the last key may be anything: its weight is 0, its value must be finite
           const int st = (2 * i + 1) % NS;

@@ -9,10 +9,10 @@
 // call, and token t belongs to the request whose token sum covers it.  So no
 // element waits for another: every block computes the sums itself (a few
 // thousand integers out of L2, about a microsecond) and then writes its share
-// of the rows and tokens -- one launch and no grid-wide step.  In-place calls
-// are safe because the only values a block may still read that the call
-// overwrites (lengths, state, the rows of finished requests) are written by
-// the block that arrives last.
+// of the rows and tokens -- one launch and no grid-wide step.  In an in-place
+// call the values that it overwrites and a block may still read (lengths,
+// state, the rows of finished requests) are written by the block that arrives
+// last.
 //
 // Bound: bytes (table rows in and out, 12 bytes a token); small steps are
 // bound by the launch and the sums' latency.
@@ -42,26 +42,29 @@ struct PagedParams {
   int32_t* requests;
 };
 
-// What request r holds and wants; lengths below zero count as zero and a row
-// never holds more pages than it has places.
+// What a request that holds c tokens and gets n more holds and wants; lengths
+// below zero count as zero and a row never holds more pages than it has places.
 struct Request {
   int held;    // pages of its row in use
   int tokens;  // new tokens
   int need;    // pages it lacks
   int back;    // pages it gives back
+  bool gone;   // it has finished
   bool fits;   // its row has places enough
 };
 
-__device__ __forceinline__ Request load_request(const PagedParams& p, int r) {
-  const int c = max(__ldcg(p.context + r), 0), n = __ldcg(p.fresh + r);
-  const int P = p.d.page_size;
+__device__ __forceinline__ Request request(const vqb_paged_desc& d, int c, int n) {
   Request q;
-  q.held = min(c > 0 ? (c - 1) / P + 1 : 0, p.d.table_width);
+  c = max(c, 0);
+  q.held = min(c > 0 ? (c - 1) / d.page_size + 1 : 0, d.table_width);
   q.tokens = max(n, 0);
-  const int64_t pages = (static_cast<int64_t>(c) + q.tokens + P - 1) / P;
-  q.fits = pages <= p.d.table_width;
-  q.need = n < 0 || !q.fits ? 0 : max(static_cast<int>(pages) - q.held, 0);
-  q.back = n < 0 ? q.held : 0;
+  const int64_t end = static_cast<int64_t>(c) + q.tokens;
+  const int64_t pages = end > 0x7fffffff ? end / d.page_size
+                                         : (end > 0 ? (static_cast<int>(end) - 1) / d.page_size + 1 : 0);
+  q.gone = n < 0;
+  q.fits = pages <= d.table_width;
+  q.need = q.gone || !q.fits ? 0 : max(static_cast<int>(pages) - q.held, 0);
+  q.back = q.gone ? q.held : 0;
   return q;
 }
 
@@ -76,59 +79,66 @@ __device__ __forceinline__ int find(const int* sums, int n, int v) {
   return lo;
 }
 
+// VEC: table rows move as 16-byte vectors
+template <bool VEC>
 __global__ void __launch_bounds__(kThreads) paged_tables_kernel(PagedParams p) {
   extern __shared__ int s_sums[];
-  const int R = p.d.n_requests;
+  const vqb_paged_desc& d = p.d;
+  const int R = d.n_requests, W = d.table_width, P = d.page_size;
   int* s_tok = s_sums;               // [R + 1] new tokens before r
   int* s_need = s_tok + R + 1;       // [R + 1] pages needed before r
   int* s_back = s_need + R + 1;      // [R + 1] pages given back before r
+  int* s_ctx = s_back + R + 1;       // [R] tokens held, [R] new tokens: read once, so that
+  int* s_new = s_ctx + R;            //     every later step is free of their latency
   __shared__ int s_warp[3][kThreads / 32];
   __shared__ int s_refused, s_given, s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_trigger();
+  const int64_t head = __ldcg(p.state), tail = __ldcg(p.state + 1);
   if (tid == 0) {
     s_refused = 0;
     s_given = 0;
   }
 
   // ---- the three sums: a thread adds up a run of requests, then the threads' totals are scanned
+  for (int r = tid; r < R; r += kThreads) {
+    s_ctx[r] = __ldcg(p.context + r);
+    s_new[r] = __ldcg(p.fresh + r);
+  }
+  __syncthreads();
+  auto load = [&](int r) { return request(d, s_ctx[r], s_new[r]); };
   const int per = (R + kThreads - 1) / kThreads;
   const int r0 = min(tid * per, R), r1 = min(r0 + per, R);
   int tot[3] = {0, 0, 0};
   for (int r = r0; r < r1; ++r) {
-    const Request q = load_request(p, r);
+    const Request q = load(r);
     tot[0] += q.tokens;
     tot[1] += q.need;
     tot[2] += q.back;
   }
-  int inc[3];
+  int inc[3] = {tot[0], tot[1], tot[2]};
+  for (int o = 1; o < 32; o <<= 1) {
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    inc[k] = tot[k];
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int k = 0; k < 3; ++k) {
       const int v = __shfl_up_sync(0xffffffffu, inc[k], o);
       if (lane >= o) inc[k] += v;
     }
-    if (lane == 31) s_warp[k][warp] = inc[k];
   }
-  __syncthreads();
-  if (warp < 3) {
-    int v = lane < kThreads / 32 ? s_warp[warp][lane] : 0;
-    const int mine = v;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    if (lane < kThreads / 32) s_warp[warp][lane] = v - mine;
+  if (lane == 31) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) s_warp[k][warp] = inc[k];
   }
   __syncthreads();
   {
     int at[3];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) at[k] = s_warp[k][warp] + inc[k] - tot[k];
+    for (int k = 0; k < 3; ++k) {
+      at[k] = inc[k] - tot[k];
+      for (int o = 0; o < warp; ++o) at[k] += s_warp[k][o];
+    }
     for (int r = r0; r < r1; ++r) {
-      const Request q = load_request(p, r);
+      const Request q = load(r);
       s_tok[r] = at[0];
       s_need[r] = at[1];
       s_back[r] = at[2];
@@ -144,16 +154,14 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(PagedParams p) {
   }
   __syncthreads();
 
-  const int64_t head = __ldcg(p.state), tail = __ldcg(p.state + 1);
-  const uint32_t F = static_cast<uint32_t>(p.d.ring_size);
-  const int returned = s_back[R];
-  const int64_t avail = tail + returned - head;
+  const uint32_t F = static_cast<uint32_t>(d.ring_size);
+  const int returned = s_back[R], total = s_tok[R];
+  const int64_t waiting = tail - head;  // entries of the ring before this call's returns
+  const int64_t avail = waiting + returned;
   const uint32_t head_mod = static_cast<uint32_t>(static_cast<uint64_t>(head) % F);
   const uint32_t tail_mod = static_cast<uint32_t>(static_cast<uint64_t>(tail) % F);
-  const int64_t waiting = tail - head;  // entries of the ring before this call's returns
-  const int W = p.d.table_width, P = p.d.page_size;
   auto taken = [&](int r, const Request& q) {
-    return q.fits && (q.need == 0 || static_cast<int64_t>(s_need[r]) + q.need <= avail);
+    return !q.gone && q.fits && (q.need == 0 || static_cast<int64_t>(s_need[r]) + q.need <= avail);
   };
   // entry `i` from the ring's start: a free page, or one given back in this call
   auto page_at = [&](int i) -> int {
@@ -165,28 +173,46 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(PagedParams p) {
     return __ldcg(p.table_in + static_cast<int64_t>(r) * W + (b - s_back[r]));
   };
   const bool table_in_place = p.table == p.table_in, ring_in_place = p.ring == p.ring_in;
+  const bool lens_in_place = p.kv_lens == p.context, state_in_place = p.state == p.state_out;
   const int gwarp = blockIdx.x * (kThreads / 32) + warp, gwarps = gridDim.x * (kThreads / 32);
-  const int64_t gthread = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
+  // tokens and ring places are dealt from the last warp down: in a small step
+  // they are other warps than those with rows, and their loads overlap
   const int64_t gthreads = static_cast<int64_t>(gridDim.x) * kThreads;
+  const int64_t gthread = gthreads - 1 - (static_cast<int64_t>(blockIdx.x) * kThreads + tid);
 
   // ---- table rows and pages given back, a warp to a request
   for (int r = gwarp; r < R; r += gwarps) {
-    const Request q = load_request(p, r);
-    const bool gone = __ldcg(p.fresh + r) < 0;
-    const bool ok = !gone && taken(r, q);
+    const Request q = load(r);
+    const bool ok = taken(r, q);
     const int32_t* in = p.table_in + static_cast<int64_t>(r) * W;
     int32_t* out = p.table + static_cast<int64_t>(r) * W;
-    if (gone) {
+    if (q.gone) {
       for (int j = lane; j < q.held; j += 32)
         p.ring[(tail_mod + static_cast<uint32_t>(s_back[r] + j)) % F] = __ldcg(in + j);
     }
-    const int keep = gone ? 0 : q.held, end = ok ? q.held + q.need : keep;
-    if (table_in_place) {
-      for (int j = keep + lane; j < end; j += 32) out[j] = page_at(s_need[r] + j - q.held);
-    } else {
-      for (int j = lane; j < W; j += 32)
-        out[j] = j < keep ? __ldcg(in + j) : (j < end ? page_at(s_need[r] + j - q.held) : -1);
+    const int keep = q.gone ? 0 : q.held;
+    if (!table_in_place) {
+      if constexpr (VEC) {
+#pragma unroll 4
+        for (int j = 4 * lane; j < W; j += 128) {
+          int4 v = make_int4(-1, -1, -1, -1);
+          if (j < keep) {
+            v = __ldcg(reinterpret_cast<const int4*>(in + j));
+            if (j + 1 >= keep) v.y = -1;
+            if (j + 2 >= keep) v.z = -1;
+            if (j + 3 >= keep) v.w = -1;
+          }
+          *reinterpret_cast<int4*>(out + j) = v;
+        }
+      } else {
+#pragma unroll 4
+        for (int j = lane; j < W; j += 32) out[j] = j < keep ? __ldcg(in + j) : -1;
+      }
+      __syncwarp();
     }
+    if (ok)
+      for (int j = lane; j < q.need; j += 32) out[q.held + j] = page_at(s_need[r] + j);
+    if (!lens_in_place && lane == 0) p.kv_lens[r] = q.gone ? 0 : max(s_ctx[r], 0) + (ok ? q.tokens : 0);
   }
   // the ring's other places (those given back in this call were written above)
   if (!ring_in_place) {
@@ -196,46 +222,51 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(PagedParams p) {
     }
   }
   // ---- tokens
-  const int total = s_tok[R];
-  for (int64_t t = gthread; t < p.d.max_tokens; t += gthreads) {
+  for (int64_t t = gthread; t < d.max_tokens; t += gthreads) {
     int slot = -1, pos = 0, r = -1;
     if (t < total) {
       r = find(s_tok, R, static_cast<int>(t));
-      const Request q = load_request(p, r);
-      const int place = max(__ldcg(p.context + r), 0) + static_cast<int>(t) - s_tok[r];
-      pos = p.d.position_offset + place;
+      const Request q = load(r);
+      const int place = max(s_ctx[r], 0) + static_cast<int>(t) - s_tok[r];
+      pos = d.position_offset + place;
       if (taken(r, q)) {
         const int col = place / P;
         const int page = col < q.held ? __ldcg(p.table_in + static_cast<int64_t>(r) * W + col)
                                       : page_at(s_need[r] + col - q.held);
-        if (page >= 0) slot = page * P + place % P;
+        if (page >= 0) slot = page * P + (place - col * P);
       }
     }
     p.slots[t] = slot;
     p.positions[t] = pos;
     p.requests[t] = r;
   }
+  if (blockIdx.x == 0)
+    for (int r = tid; r <= R; r += kThreads) p.cu_q[r] = s_tok[r];
 
-  // ---- the block that arrives last has no reader left beside it
-  __syncthreads();
-  if (tid == 0) {
-    __threadfence();
-    const unsigned long long n = atomicAdd(reinterpret_cast<unsigned long long*>(p.state + 3), 1ull);
-    s_last = n == gridDim.x - 1;
+  // ---- what is written over what other blocks may still read: by the block that
+  // arrives last (none but this one when the grid is one block)
+  const bool over = table_in_place || lens_in_place || state_in_place;
+  if (over && gridDim.x > 1) {
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      const unsigned long long n = atomicAdd(reinterpret_cast<unsigned long long*>(p.state + 3), 1ull);
+      s_last = n == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
+  } else {
+    if (blockIdx.x != 0) return;
+    __syncthreads();
   }
-  __syncthreads();
-  if (!s_last) return;
   int refused = 0, given = 0;
   for (int r = tid; r < R; r += kThreads) {
-    const Request q = load_request(p, r);
-    const bool gone = __ldcg(p.fresh + r) < 0;
-    const bool ok = !gone && taken(r, q);
-    const int c = max(__ldcg(p.context + r), 0);
-    if (!gone && !ok) ++refused;
+    const Request q = load(r);
+    const bool ok = taken(r, q);
+    if (!q.gone && !ok) ++refused;
     if (ok) given += q.need;
-    p.kv_lens[r] = gone ? 0 : (ok ? c + q.tokens : c);
+    if (lens_in_place) p.kv_lens[r] = q.gone ? 0 : max(s_ctx[r], 0) + (ok ? q.tokens : 0);
   }
-  for (int r = tid; r <= R; r += kThreads) p.cu_q[r] = s_tok[r];
   if (refused) atomicAdd(&s_refused, refused);
   if (given) atomicAdd(&s_given, given);
   if (table_in_place) {
@@ -246,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(PagedParams p) {
   }
   __syncthreads();
   if (tid == 0) {
-    p.state[3] = 0;
+    if (over && gridDim.x > 1) p.state[3] = 0;
     p.state_out[0] = head + s_given;
     p.state_out[1] = tail + returned;
     p.state_out[2] = s_refused;
@@ -284,12 +315,15 @@ extern "C" vqb_status vqb_paged_tables(const vqb_paged_desc* desc, const int32_t
   blocks = blocks > others ? blocks : others;
   blocks = blocks > places ? blocks : places;
   blocks = blocks < 1 ? 1 : (blocks > di.sms ? di.sms : blocks);
-  const size_t smem = 3 * sizeof(int) * (static_cast<size_t>(d.n_requests) + 1);
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(paged_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  const size_t smem = sizeof(int) * (5 * static_cast<size_t>(d.n_requests) + 3);
+  const bool vec = d.table_width % 4 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(block_table) | reinterpret_cast<uintptr_t>(block_table_out)) & 15) == 0;
+  const auto kern = vec ? paged_tables_kernel<true> : paged_tables_kernel<false>;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
-  if (launch_pdl(paged_tables_kernel, static_cast<unsigned>(blocks), kThreads, smem,
-                 reinterpret_cast<cudaStream_t>(stream), p) != cudaSuccess)
+  if (launch_pdl(kern, static_cast<unsigned>(blocks), kThreads, smem, reinterpret_cast<cudaStream_t>(stream), p) !=
+      cudaSuccess)
     return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
