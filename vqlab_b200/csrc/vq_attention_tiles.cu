@@ -12,10 +12,11 @@
 //     tensor memory, then O_t += P_t V with P_t in tensor memory over S_t's
 //     columns and V read along its other dimension.  Order: P0 V, Q0 K'^T, P1 V,
 //     Q1 K'^T: while one tile's softmax runs, the other's products do;
-//   * four softmax warps a tile, a thread a row: the row's 128 scores into
-//     registers, running maximum and sum, weights as 16-bit numbers back to
-//     tensor memory.  O is rescaled in place, by the same thread, only when the
-//     maximum has grown by more than 2^kSlack.
+//   * eight softmax warps a tile, two threads a row: each takes 64 of the row's
+//     scores into registers, they agree on the running maximum through shared
+//     memory, and write their weights as 16-bit numbers back to tensor memory.
+//     O is rescaled in place, half of it by each thread, only when the maximum
+//     has grown by more than 2^kSlack.
 // Scores, weights' sum and O are fp32; the weights are rounded once to the
 // cache's type, which the MMA needs.
 //
@@ -28,13 +29,13 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-constexpr int kThreads = 320;
-constexpr int kWarpMma = 8, kWarpTma = 9;
+constexpr int kThreads = 576;
+constexpr int kWarpMma = 16, kWarpTma = 17;
 constexpr int kTmemCols = 512;
 template <int D>
 constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
 template <int D>
-constexpr int kStages = D == 128 ? 5 : 8;
+constexpr int kStages = D == 128 ? 4 : 8;
 template <int D>
 constexpr size_t tiles_smem() {
   return 1024 + size_t(2) * kTileRows * D * 2 + size_t(kStages<D>) * kStageBytes<D> + 256;
@@ -42,25 +43,29 @@ constexpr size_t tiles_smem() {
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                :: "r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // D (+)= A B, A and B in shared memory
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // D (+)= A B, A in tensor memory
 __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0) : "memory");
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 #define VQB_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
 #define VQB_RW8(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7])
@@ -75,16 +80,18 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* v) {
 __device__ __forceinline__ void tc_wait_ld32(uint32_t* v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : VQB_RW8(v, 0), VQB_RW8(v, 8), VQB_RW8(v, 16), VQB_RW8(v, 24)::"memory");
 }
+__device__ __forceinline__ void tc_wait_ld16(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : VQB_RW8(v, 0), VQB_RW8(v, 8)::"memory");
+}
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       :: "r"(addr), VQB_S8(v, 0), VQB_S8(v, 8) : "memory");
 }
-__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t* v) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      :: "r"(addr), VQB_S8(v, 0), VQB_S8(v, 8), VQB_S8(v, 16), VQB_S8(v, 24) : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : VQB_R8(v, 0), VQB_R8(v, 8) : "r"(addr) : "memory");
 }
 
 // pairs of fp32 numbers
@@ -114,56 +121,38 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// The scores of a row's 128 keys at tensor-memory address `addr`, 32 at a time,
-// the next 32 on their way while `use(chunk, scores)` works on these.  MASK:
-// scores from `lim` on become -inf.
-template <bool MASK, typename F>
-__device__ __forceinline__ void for_scores(uint32_t addr, int lim, F use) {
-  uint32_t a[32], b[32];
-  tc_ld32(addr, a);
+// The largest of 64 scores.
+__device__ __forceinline__ float max64(const float* s) {
+  float t[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t* v = (c & 1) ? b : a;
-    tc_wait_ld32(v);
-    if (c < 3) tc_ld32(addr + (c + 1) * 32, (c & 1) ? a : b);
-    if constexpr (MASK) {
+  for (int k = 0; k < 4; ++k) t[k] = max3(s[16 * k], s[16 * k + 1], s[16 * k + 2]);
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if (c * 32 + e >= lim) v[e] = 0xFF800000u;
-    }
-    use(c, reinterpret_cast<const float*>(v));
-  }
+  for (int e = 3; e < 15; e += 2)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = max3(t[k], s[16 * k + e], s[16 * k + e + 1]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], s[16 * k + 15]);
+  return fmaxf(max3(t[0], t[1], t[2]), t[3]);
 }
-template <bool MASK>
-__device__ __forceinline__ float scores_max(uint32_t addr, int lim) {
-  float t0 = -INFINITY, t1 = -INFINITY;
-  for_scores<MASK>(addr, lim, [&](int, const float* s) {
-#pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      t0 = max3(t0, s[e], s[e + 1]);
-      t1 = max3(t1, s[e + 2], s[e + 3]);
-    }
-  });
-  return fmaxf(t0, t1);
-}
-// Weights 2^(score * scale - base) of the row's keys: to `addr` as 16-bit numbers,
-// over scores already read; returns their sum.
-template <bool MASK, bool BF16>
-__device__ __forceinline__ float scores_weights(uint32_t addr, int lim, float scale, float base) {
+// Weights 2^(score * scale - base) of 64 scores: to tensor memory at `addr` as
+// 16-bit numbers; returns their sum.
+template <bool BF16>
+__device__ __forceinline__ float weights64(uint32_t addr, const float* s, float scale, float base) {
   const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
   uint64_t sum0 = pair(0.f, 0.f), sum1 = sum0;
-  for_scores<MASK>(addr, lim, [&](int c, const float* s) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
     uint32_t pk[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float2 x = unpair(fma2(pair(s[2 * e], s[2 * e + 1]), scale2, base2));
+      const float2 x = unpair(fma2(pair(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), scale2, base2));
       const float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
       if (e & 1) sum1 = add2(sum1, pair(w.x, w.y));
       else sum0 = add2(sum0, pair(w.x, w.y));
       pk[e] = pack16<BF16>(w.x, w.y);
     }
     tc_st16(addr + c * 16, pk);
-  });
+  }
   const float2 t = unpair(add2(sum0, sum1));
   return t.x + t.y;
 }
@@ -248,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char smem_raw[];
+  __shared__ float s_half[2][2][2][kTileRows];  // [turn][tile][half]: the halves' maxima, at the end their sums
   constexpr int NS = kStages<D>;
   constexpr int kHalf = kTileKeys * 128;  // 64 elements of 128 rows
   constexpr int kQTile = kTileRows * D * 2;
@@ -258,12 +248,13 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   uint64_t* kv_full = bars;            // [NS] the stage's copies landed
   uint64_t* kv_empty = bars + NS;      // [NS] the MMAs that read the stage are done
   uint64_t* s_full = kv_empty + NS;    // [2] a tile's scores are in tensor memory
-  uint64_t* p_full = s_full + 2;       // [2] its weights are (four warps)
+  uint64_t* p_full = s_full + 2;       // [2] its weights are (eight warps)
   uint64_t* o_full = p_full + 2;       // [2] its O has this key tile
   uint64_t* mma_done = o_full + 2;     // [1] teardown
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // values that every lane has alike are broadcast, so that the MMA warp's operands are uniform
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const vqb_attention_desc& d = p.d;
 
   if (threadIdx.x == 0) {
@@ -273,7 +264,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[t], 8);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(mma_done, 1);
@@ -284,13 +275,13 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   clear_status(p, pass);
   pdl_trigger();
   TileWork w;
-  if (!find_work(p, pass, blockIdx.x, lane, &w)) return;  // the same for every thread
+  if (!find_work(p, pass, blockIdx.x / d.kv_heads, lane, &w)) return;  // the same for every thread
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const int kvh = blockIdx.y, split = blockIdx.z;
+  const int kvh = blockIdx.x % d.kv_heads, split = blockIdx.y;
   const int tiles0 = (w.seg0 + kTileKeys - 1) / kTileKeys, all = tiles0 + (w.seg1 + kTileKeys - 1) / kTileKeys;
   const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / pass.splits);
   const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / pass.splits) - t0;
@@ -313,7 +304,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   // the columns of tile t's scores (its weights lie over them) and output
   auto s_col = [&](int t) { return tmem + t * kTileKeys; };
   auto o_col = [&](int t) { return tmem + 2 * kTileKeys + t * D; };
@@ -360,78 +351,125 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
     if (lane == 0)
       for (int k = max(issued - NS, 0); k < issued; ++k) mbar_drain(&kv_full[k % NS], (k / NS) & 1);
   } else if (warp == kWarpMma) {
-    // ---------------- the MMAs, one thread
-    if (lane == 0 && n > 0) {
-      constexpr uint32_t qk = idesc_f16<BF16>(kTileKeys, false), pv = idesc_f16<BF16>(D, true);
-      auto stage = [&](int idx) { return smem_u32(ring + (idx % NS) * kStageBytes<D>); };
-      auto wait_kv = [&](int idx) { return mbar_wait(&kv_full[idx % NS], (idx / NS) & 1, abort_flag); };
-      auto mma_qk = [&](int t, int i) {
-        const uint32_t qa = smem_u32(q_s + t * kQTile), kb = stage(2 * i);
+    // ---------------- the MMAs: the warp waits together, one thread issues
+    constexpr uint32_t qk = idesc_f16<BF16>(kTileKeys, false), pv = idesc_f16<BF16>(D, true);
+    const bool issuer = elect_one();
+    const uint32_t q0 = smem_u32(q_s), ring0 = smem_u32(ring);
+    auto wait_kv = [&](int idx) { return warp_wait(&kv_full[idx % NS], (idx / NS) & 1, abort_flag); };
+    // S_t = Q_t K^T: 16 of D a step; 64 are 128 contiguous bytes of each row
+    auto mma_qk = [&](int t, int i) {
+      const uint64_t a = desc128(q0 + t * kQTile, 16), b = desc128(ring0 + ((2 * i) % NS) * kStageBytes<D>, 16);
+      if (issuer) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
-          tc_mma_ss(s_col(t), desc128(qa + off, 16), desc128(kb + off, 16), qk, ks > 0);
+          const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
+          tc_mma_ss(s_col(t), a + off, b + off, qk, ks > 0);
         }
         tc_commit(&s_full[t]);
-      };
-      auto held_of = [&](int i) {
-        const bool own = t0 + i >= tiles0;
-        return min((own ? w.seg1 : w.seg0) - (own ? t0 + i - tiles0 : t0 + i) * kTileKeys, kTileKeys);
-      };
-      bool ok = wait_kv(0);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < active; ++t) mma_qk(t, 0);
-        tc_commit(&kv_empty[0]);
       }
-      for (int i = 0; i < n && ok; ++i) {
-        const int steps = (held_of(i) + 15) / 16;
-        for (int t = 0; t < active && ok; ++t) {
-          ok = mbar_wait(&p_full[t], i & 1, abort_flag) && (t > 0 || wait_kv(2 * i + 1));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t vb = stage(2 * i + 1);
-          for (int ks = 0; ks < steps; ++ks)
-            tc_mma_ts(o_col(t), s_col(t) + ks * 8, desc128(vb + ks * 2048, kHalf), pv, i > 0 || ks > 0);
-          tc_commit(&o_full[t]);
-          if (i + 1 < n) {
-            if (t == 0) {
-              ok = wait_kv(2 * i + 2);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            mma_qk(t, i + 1);
-          }
+      __syncwarp();
+    };
+    // O_t (+)= P_t V: 16 keys a step, up to the last that is held
+    auto mma_pv = [&](int t, int i) {
+      const bool own = t0 + i >= tiles0;
+      const int held = (own ? w.seg1 : w.seg0) - (own ? t0 + i - tiles0 : t0 + i) * kTileKeys;
+      const uint64_t b = desc128(ring0 + ((2 * i + 1) % NS) * kStageBytes<D>, kHalf);
+      if (issuer) {
+        if (held >= kTileKeys) {
+          tc_mma_ts(o_col(t), s_col(t), b, pv, i > 0);
+#pragma unroll
+          for (int ks = 1; ks < 8; ++ks) tc_mma_ts(o_col(t), s_col(t) + ks * 8, b + ks * (2048 >> 4), pv, 1);
+        } else {
+          for (int ks = 0; ks < (held + 15) / 16; ++ks)
+            tc_mma_ts(o_col(t), s_col(t) + ks * 8, b + ks * (2048 >> 4), pv, i > 0 || ks > 0);
         }
-        if (!ok) break;
-        tc_commit(&kv_empty[(2 * i + 1) % NS]);
-        if (i + 1 < n) tc_commit(&kv_empty[(2 * i + 2) % NS]);
+        tc_commit(&o_full[t]);
       }
-      tc_commit(mma_done);
-      mbar_drain(mma_done, 0);
+      __syncwarp();
+    };
+    auto release = [&](int idx) {
+      if (issuer) tc_commit(&kv_empty[idx % NS]);
+      __syncwarp();
+    };
+    bool ok = n > 0 && wait_kv(0);
+    if (ok) {
+      tc_fence_after();
+      mma_qk(0, 0);
+      if (active > 1) mma_qk(1, 0);
+      release(0);
+    }
+    for (int i = 0; i < n && ok; ++i) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (t == 1 && active < 2) break;
+        ok = ok && warp_wait(&p_full[t], i & 1, abort_flag) && (t > 0 || wait_kv(2 * i + 1));
+        if (!ok) break;
+        tc_fence_after();
+        mma_pv(t, i);
+        if (i + 1 < n) {
+          if (t == 0) {
+            if (!(ok = wait_kv(2 * i + 2))) break;
+            tc_fence_after();
+          }
+          mma_qk(t, i + 1);
+        }
+      }
+      if (!ok) break;
+      release(2 * i + 1);
+      if (i + 1 < n) release(2 * i + 2);
+    }
+    if (n > 0) {
+      if (issuer) {
+        tc_commit(mma_done);
+        mbar_drain(mma_done, 0);
+      }
+      __syncwarp();
     }
   } else {
-    // ---------------- softmax: a thread a row
-    const int t = warp >> 2;
+    // ---------------- softmax: two threads a row, 64 keys of a tile each
+    const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
     if (t < active) {
-      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const int g = w.row0 + t * kTileRows + (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+      const int row = quad * 32 + lane;
+      const int g = w.row0 + t * kTileRows + row;
       const int gv = min(g, w.rows - 1), tok = gv / p.group;
       const int vis = pass.joint ? 0 : visible(p, w.rq, tok);
+      const uint32_t srow = s_col(t) + lanes + half * 64, prow = s_col(t) + lanes + half * 32;
+      const uint32_t orow = o_col(t) + lanes + half * (D / 2);
+      // the row's two warps meet once a key tile, whatever happens to their waits
+      auto meet = [&] { asm volatile("barrier.cta.sync %0, 64;" :: "r"(1 + t * 4 + quad) : "memory"); };
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
       for (int i = 0; i < n; ++i) {
         const bool own = t0 + i >= tiles0;
         const int start = (own ? t0 + i - tiles0 : t0 + i) * kTileKeys;
         const int held = min((own ? w.seg1 : w.seg0) - start, kTileKeys);
-        const int lim = own ? vis - start : held;
-        if (!(ok = warp_wait(&s_full[t], i & 1, abort_flag))) break;
+        const int lim = (own ? vis - start : held) - half * 64;
+        ok = ok && warp_wait(&s_full[t], i & 1, abort_flag);
         // the MMAs of the key tile before this one came first: done already, waited for to keep in step with the barrier
-        if (i > 0 && !(ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag))) break;
+        if (i > 0) ok = ok && warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
+        float s[64];
+        float mine = -INFINITY;
+        if (ok) {
+          tc_fence_after();
+          uint32_t* u = reinterpret_cast<uint32_t*>(s);
+          tc_ld32(srow, u);
+          tc_ld32(srow + 32, u + 32);
+          tc_wait_ld32(u);
+          tc_wait_ld32(u + 32);
+          if (__any_sync(0xffffffffu, lim < 64)) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (c >= lim) s[c] = -INFINITY;
+          }
+          mine = max64(s);
+        }
+        s_half[i & 1][t][half][row] = mine;
+        tc_fence_before();
+        meet();
         tc_fence_after();
-        const uint32_t srow = s_col(t) + lanes;
-        const bool mask = __any_sync(0xffffffffu, lim < kTileKeys);
-        const float mx = (mask ? scores_max<true>(srow, lim) : scores_max<false>(srow, lim)) * p.scale_log2;
+        if (!ok) continue;
+        const float mx = fmaxf(mine, s_half[i & 1][t][half ^ 1][row]) * p.scale_log2;
         if (__any_sync(0xffffffffu, mx > m + kSlack)) {
           const float mn = fmaxf(m, mx);
           const float f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
@@ -440,22 +478,22 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
           if (i > 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tc_ld32(o_col(t) + lanes + c * 32, o);
-              tc_wait_ld();
+              uint32_t o[16];
+              tc_ld16(orow + c * 16, o);
+              tc_wait_ld16(o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tc_st32(o_col(t) + lanes + c * 32, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc_st16(orow + c * 16, o);
             }
           }
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        l += mask ? scores_weights<true, BF16>(srow, lim, p.scale_log2, base)
-                  : scores_weights<false, BF16>(srow, lim, p.scale_log2, base);
-        if (t == 0 && (warp & 3) == 0 && (held & 15)) {
+        // over the scores: both halves have been read by now
+        l += weights64<BF16>(prow, s, p.scale_log2, base);
+        if (t == 0 && half == 0 && quad == 0 && (held & 15)) {
           // what lies past the last key may be anything: its weight is 0, its value must be finite
           const int st = (2 * i + 1) % NS;
-          if (!(ok = warp_wait(&kv_full[st], ((2 * i + 1) / NS) & 1, abort_flag))) break;
+          if (!(ok = warp_wait(&kv_full[st], ((2 * i + 1) / NS) & 1, abort_flag))) continue;
           const int first = held, rows = ((held + 15) & ~15) - held;
           for (int e = lane; e < rows * (D / 8); e += 32) {
             const int rr = first + e / (D / 8), c = e % (D / 8);
@@ -469,7 +507,11 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
-      if (ok && n > 0) ok = warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
+      if (n > 0) ok = ok && warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
+      // the row's sum is both halves'
+      s_half[n & 1][t][half][row] = l;
+      meet();
+      l += s_half[n & 1][t][half ^ 1][row];
       if (!ok && lane == 0) *p.status = VQB_TIMEOUT;
       if (ok) {
         tc_fence_after();
@@ -481,17 +523,18 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         const int64_t at = (pass.part0 + split) * (static_cast<int64_t>(d.n_tokens) * d.heads) + grow;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < D / 64; ++c) {
           uint32_t o[32];
           if (n > 0) {
-            tc_ld32(o_col(t) + lanes + c * 32, o);
-            tc_wait_ld();
+            tc_ld32(orow + c * 32, o);
+            tc_wait_ld32(o);
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
+          const int col = half * (D / 2) + c * 32;
           if (live && partial) {
-            uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + c * 32);
+            uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + col);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else if (live) {
@@ -499,13 +542,13 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               pk[e] = pack16<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-            uint4* dst = reinterpret_cast<uint4*>(p.out + token * d.out_token_stride + head * d.out_head_stride + c * 32);
+            uint4* dst = reinterpret_cast<uint4*>(p.out + token * d.out_token_stride + head * d.out_head_stride + col);
 #pragma unroll
             for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
           }
           __syncwarp();
         }
-        if (live) {
+        if (live && half == 0) {
           if (partial) p.part_ml[at] = make_float2(m, l);
           else if (p.lse) p.lse[grow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
@@ -522,11 +565,12 @@ template <int D, bool BF16>
 vqb_status launch(const AttnParams& p, const AttnPass& pass, unsigned tiles, const CUtensorMap& km, const CUtensorMap& vm,
                   cudaStream_t s) {
   constexpr size_t smem = tiles_smem<D>();
-  static_assert(smem <= 232448, "over the opt-in shared memory of an SM");
+  static_assert(smem + 4096 <= 232448, "over the opt-in shared memory of an SM");
   if (cudaFuncSetAttribute(attention_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
-  const dim3 grid(tiles, p.d.kv_heads, pass.splits);
+  // the rows with the most keys first, over all heads
+  const dim3 grid(tiles * p.d.kv_heads, pass.splits);
   if (launch_pdl(attention_tiles_kernel<D, BF16>, grid, kThreads, smem, s, p, pass, km, vm) != cudaSuccess)
     return VQB_CUDA_ERROR;
   note_launch();
