@@ -8,15 +8,19 @@
 // tile of 128 keys.  Roles:
 //   * a TMA warp fills a ring of shared-memory stages with K and V tiles, one
 //     box a page and 64 elements (a lane a page);
-//   * one thread issues the MMAs: S_t = Q_t K^T (both from shared memory) into
-//     tensor memory, then O_t += P_t V with P_t in tensor memory over S_t's
-//     columns and V read along its other dimension.  Order: P0 V, Q0 K'^T, P1 V,
-//     Q1 K'^T: while one tile's softmax runs, the other's products do;
-//   * eight softmax warps a tile, two threads a row: each takes 64 of the row's
-//     scores into registers, they agree on the running maximum through shared
-//     memory, and write their weights as 16-bit numbers back to tensor memory.
-//     O is rescaled in place, half of it by each thread, only when the maximum
+//   * one thread issues the MMAs: S = Q_t K^T (both from shared memory) into
+//     tensor memory, then O_t += P_t V with P_t in tensor memory and V read along
+//     its other dimension;
+//   * four softmax warps a tile, a thread a row: the row's 128 scores into
+//     registers, running maximum and sum, weights as 16-bit numbers to tensor
+//     memory.  O is rescaled in place, by the same thread, only when the maximum
 //     has grown by more than 2^kSlack.
+// Tensor memory's 512 columns hold two O tiles (256), two weight tiles (128) and
+// one score tile (128) that the two row tiles use in turn: it is free again as
+// soon as the scores are in registers, so the next Q K^T runs beside this tile's
+// exponentials and no score waits for a P V.  (With a score tile each, weights
+// had to lie over scores, and each tile's chain of exponentials, P V and Q K^T was
+// serial: 3900 cycles a key tile against 2100 of MMAs.)
 // Scores, weights' sum and O are fp32; the weights are rounded once to the
 // cache's type, which the MMA needs.
 //
@@ -29,13 +33,13 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-constexpr int kThreads = 576;
-constexpr int kWarpMma = 16, kWarpTma = 17;
+constexpr int kThreads = 320;
+constexpr int kWarpMma = 8, kWarpTma = 9;
 constexpr int kTmemCols = 512;
 template <int D>
 constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
 template <int D>
-constexpr int kStages = D == 128 ? 4 : 8;
+constexpr int kStages = D == 128 ? 5 : 8;
 template <int D>
 constexpr size_t tiles_smem() {
   return 1024 + size_t(2) * kTileRows * D * 2 + size_t(kStages<D>) * kStageBytes<D> + 256;
@@ -121,37 +125,30 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// The largest of 64 scores.
-__device__ __forceinline__ float max64(const float* s) {
+// The largest of 128 scores.
+__device__ __forceinline__ float max128(const float* s) {
   float t[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) t[k] = max3(s[16 * k], s[16 * k + 1], s[16 * k + 2]);
+  for (int k = 0; k < 4; ++k) t[k] = max3(s[32 * k], s[32 * k + 1], s[32 * k + 2]);
 #pragma unroll
-  for (int e = 3; e < 15; e += 2)
+  for (int e = 3; e < 31; e += 2)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) t[k] = max3(t[k], s[16 * k + e], s[16 * k + e + 1]);
+    for (int k = 0; k < 4; ++k) t[k] = max3(t[k], s[32 * k + e], s[32 * k + e + 1]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], s[16 * k + 15]);
+  for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], s[32 * k + 31]);
   return fmaxf(max3(t[0], t[1], t[2]), t[3]);
 }
-// Weights 2^(score * scale - base) of 64 scores: to tensor memory at `addr` as
-// 16-bit numbers; returns their sum.
+// Weights 2^(score * scale - base) of 32 scores as 16-bit numbers; returns their sum.
 template <bool BF16>
-__device__ __forceinline__ float weights64(uint32_t addr, const float* s, float scale, float base) {
-  const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+__device__ __forceinline__ float weights32(uint32_t (&pk)[16], const float* s, uint64_t scale2, uint64_t base2) {
   uint64_t sum0 = pair(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t pk[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float2 x = unpair(fma2(pair(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), scale2, base2));
-      const float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-      if (e & 1) sum1 = add2(sum1, pair(w.x, w.y));
-      else sum0 = add2(sum0, pair(w.x, w.y));
-      pk[e] = pack16<BF16>(w.x, w.y);
-    }
-    tc_st16(addr + c * 16, pk);
+  for (int e = 0; e < 16; ++e) {
+    const float2 x = unpair(fma2(pair(s[2 * e], s[2 * e + 1]), scale2, base2));
+    const float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+    if (e & 1) sum1 = add2(sum1, pair(w.x, w.y));
+    else sum0 = add2(sum0, pair(w.x, w.y));
+    pk[e] = pack16<BF16>(w.x, w.y);
   }
   const float2 t = unpair(add2(sum0, sum1));
   return t.x + t.y;
@@ -237,7 +234,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ float s_half[2][2][2][kTileRows];  // [turn][tile][half]: the halves' maxima, at the end their sums
   constexpr int NS = kStages<D>;
   constexpr int kHalf = kTileKeys * 128;  // 64 elements of 128 rows
   constexpr int kQTile = kTileRows * D * 2;
@@ -248,7 +244,8 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   uint64_t* kv_full = bars;            // [NS] the stage's copies landed
   uint64_t* kv_empty = bars + NS;      // [NS] the MMAs that read the stage are done
   uint64_t* s_full = kv_empty + NS;    // [2] a tile's scores are in tensor memory
-  uint64_t* p_full = s_full + 2;       // [2] its weights are (eight warps)
+  uint64_t* s_read = s_full + 2;       // [2] they are in registers (four warps)
+  uint64_t* p_full = s_read + 2;       // [2] its weights are in tensor memory (four warps)
   uint64_t* o_full = p_full + 2;       // [2] its O has this key tile
   uint64_t* mma_done = o_full + 2;     // [1] teardown
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
@@ -264,7 +261,8 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 8);
+      mbar_init(&s_read[t], 4);
+      mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(mma_done, 1);
@@ -305,8 +303,9 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  // the columns of tile t's scores (its weights lie over them) and output
-  auto s_col = [&](int t) { return tmem + t * kTileKeys; };
+  // columns: the scores of either tile, tile t's weights, its output
+  const uint32_t s_col = tmem;
+  auto p_col = [&](int t) { return tmem + kTileKeys + t * (kTileKeys / 2); };
   auto o_col = [&](int t) { return tmem + 2 * kTileKeys + t * D; };
 
   if (warp == kWarpTma) {
@@ -363,7 +362,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
-          tc_mma_ss(s_col(t), a + off, b + off, qk, ks > 0);
+          tc_mma_ss(s_col, a + off, b + off, qk, ks > 0);
         }
         tc_commit(&s_full[t]);
       }
@@ -376,12 +375,12 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       const uint64_t b = desc128(ring0 + ((2 * i + 1) % NS) * kStageBytes<D>, kHalf);
       if (issuer) {
         if (held >= kTileKeys) {
-          tc_mma_ts(o_col(t), s_col(t), b, pv, i > 0);
+          tc_mma_ts(o_col(t), p_col(t), b, pv, i > 0);
 #pragma unroll
-          for (int ks = 1; ks < 8; ++ks) tc_mma_ts(o_col(t), s_col(t) + ks * 8, b + ks * (2048 >> 4), pv, 1);
+          for (int ks = 1; ks < 8; ++ks) tc_mma_ts(o_col(t), p_col(t) + ks * 8, b + ks * (2048 >> 4), pv, 1);
         } else {
           for (int ks = 0; ks < (held + 15) / 16; ++ks)
-            tc_mma_ts(o_col(t), s_col(t) + ks * 8, b + ks * (2048 >> 4), pv, i > 0 || ks > 0);
+            tc_mma_ts(o_col(t), p_col(t) + ks * 8, b + ks * (2048 >> 4), pv, i > 0 || ks > 0);
         }
         tc_commit(&o_full[t]);
       }
@@ -391,33 +390,39 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       if (issuer) tc_commit(&kv_empty[idx % NS]);
       __syncwarp();
     };
+    // Q0 K'^T, P1 V, Q1 K'^T, P0 V in turn: a tile's scores are computed while its
+    // softmax warps still work on the weights of the key tile before
+    auto wait_bar = [&](uint64_t* bar, int i) {
+      const bool r = warp_wait(bar, i & 1, abort_flag);
+      tc_fence_after();
+      return r;
+    };
+    const int last = active - 1;
     bool ok = n > 0 && wait_kv(0);
     if (ok) {
       tc_fence_after();
       mma_qk(0, 0);
-      if (active > 1) mma_qk(1, 0);
-      release(0);
     }
     for (int i = 0; i < n && ok; ++i) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (t == 1 && active < 2) break;
-        ok = ok && warp_wait(&p_full[t], i & 1, abort_flag) && (t > 0 || wait_kv(2 * i + 1));
-        if (!ok) break;
-        tc_fence_after();
-        mma_pv(t, i);
-        if (i + 1 < n) {
-          if (t == 0) {
-            if (!(ok = wait_kv(2 * i + 2))) break;
-            tc_fence_after();
-          }
-          mma_qk(t, i + 1);
-        }
+      if (active > 1) {
+        if (!(ok = wait_bar(&s_read[0], i))) break;
+        mma_qk(1, i);
       }
-      if (!ok) break;
-      release(2 * i + 1);
-      if (i + 1 < n) release(2 * i + 2);
+      release(2 * i);
+      if (active > 1 && i > 0) {
+        if (!(ok = wait_bar(&p_full[1], i - 1))) break;
+        mma_pv(1, i - 1);
+        release(2 * i - 1);
+      }
+      if (i + 1 < n) {
+        if (!(ok = wait_kv(2 * i + 2) && wait_bar(&s_read[last], i))) break;
+        mma_qk(0, i + 1);
+      }
+      if (!(ok = wait_kv(2 * i + 1) && wait_bar(&p_full[0], i))) break;
+      mma_pv(0, i);
+      if (active == 1) release(2 * i + 1);
     }
+    if (ok && active > 1 && (ok = wait_bar(&p_full[1], n - 1))) mma_pv(1, n - 1);
     if (n > 0) {
       if (issuer) {
         tc_commit(mma_done);
@@ -426,58 +431,51 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       __syncwarp();
     }
   } else {
-    // ---------------- softmax: two threads a row, 64 keys of a tile each
-    const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+    // ---------------- softmax: a thread a row
+    const int t = warp >> 2;
     if (t < active) {
-      const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-      const int row = quad * 32 + lane;
-      const int g = w.row0 + t * kTileRows + row;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const int g = w.row0 + t * kTileRows + (warp & 3) * 32 + lane;
       const int gv = min(g, w.rows - 1), tok = gv / p.group;
       const int vis = pass.joint ? 0 : visible(p, w.rq, tok);
-      const uint32_t srow = s_col(t) + lanes + half * 64, prow = s_col(t) + lanes + half * 32;
-      const uint32_t orow = o_col(t) + lanes + half * (D / 2);
-      // the row's two warps meet once a key tile, whatever happens to their waits
-      auto meet = [&] { asm volatile("barrier.cta.sync %0, 64;" :: "r"(1 + t * 4 + quad) : "memory"); };
+      const uint32_t srow = s_col + lanes, prow = p_col(t) + lanes, orow = o_col(t) + lanes;
+      const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
       for (int i = 0; i < n; ++i) {
         const bool own = t0 + i >= tiles0;
         const int start = (own ? t0 + i - tiles0 : t0 + i) * kTileKeys;
         const int held = min((own ? w.seg1 : w.seg0) - start, kTileKeys);
-        const int lim = (own ? vis - start : held) - half * 64;
-        ok = ok && warp_wait(&s_full[t], i & 1, abort_flag);
-        // the MMAs of the key tile before this one came first: done already, waited for to keep in step with the barrier
-        if (i > 0) ok = ok && warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
-        float s[64];
-        float mine = -INFINITY;
-        if (ok) {
-          tc_fence_after();
-          uint32_t* u = reinterpret_cast<uint32_t*>(s);
-          tc_ld32(srow, u);
-          tc_ld32(srow + 32, u + 32);
-          tc_wait_ld32(u);
-          tc_wait_ld32(u + 32);
-          if (__any_sync(0xffffffffu, lim < 64)) {
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c >= lim) s[c] = -INFINITY;
-          }
-          mine = max64(s);
-        }
-        s_half[i & 1][t][half][row] = mine;
-        tc_fence_before();
-        meet();
+        const int lim = own ? vis - start : held;
+        if (!(ok = warp_wait(&s_full[t], i & 1, abort_flag))) break;
         tc_fence_after();
-        if (!ok) continue;
-        const float mx = fmaxf(mine, s_half[i & 1][t][half ^ 1][row]) * p.scale_log2;
+        float s[128];
+        uint32_t* u = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc_ld32(srow + c * 32, u + c * 32);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc_wait_ld32(u + c * 32);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_read[t]);
+        if (__any_sync(0xffffffffu, lim < kTileKeys)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c >= lim) s[c] = -INFINITY;
+        }
+        const float mx = max128(s) * p.scale_log2;
+        bool fresh = i == 0;  // the weights of the key tile before have met their values
         if (__any_sync(0xffffffffu, mx > m + kSlack)) {
           const float mn = fmaxf(m, mx);
           const float f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
           m = mn;
           l *= f;
           if (i > 0) {
+            if (!(ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag))) break;
+            fresh = true;
+            tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
               tc_ld16(orow + c * 16, o);
               tc_wait_ld16(o);
@@ -488,12 +486,24 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
           }
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        // over the scores: both halves have been read by now
-        l += weights64<BF16>(prow, s, p.scale_log2, base);
-        if (t == 0 && half == 0 && quad == 0 && (held & 15)) {
+        const uint64_t base2 = pair(-base, -base);
+        uint32_t pk0[16], pk1[16];
+        l += weights32<BF16>(pk0, s, scale2, base2);
+        l += weights32<BF16>(pk1, s + 32, scale2, base2);
+        if (!fresh) {
+          if (!(ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag))) break;
+          tc_fence_after();
+        }
+        tc_st16(prow, pk0);
+        tc_st16(prow + 16, pk1);
+        l += weights32<BF16>(pk0, s + 64, scale2, base2);
+        tc_st16(prow + 32, pk0);
+        l += weights32<BF16>(pk1, s + 96, scale2, base2);
+        tc_st16(prow + 48, pk1);
+        if (t == 0 && (warp & 3) == 0 && (held & 15)) {
           // what lies past the last key may be anything: its weight is 0, its value must be finite
           const int st = (2 * i + 1) % NS;
-          if (!(ok = warp_wait(&kv_full[st], ((2 * i + 1) / NS) & 1, abort_flag))) continue;
+          if (!(ok = warp_wait(&kv_full[st], ((2 * i + 1) / NS) & 1, abort_flag))) break;
           const int first = held, rows = ((held + 15) & ~15) - held;
           for (int e = lane; e < rows * (D / 8); e += 32) {
             const int rr = first + e / (D / 8), c = e % (D / 8);
@@ -507,11 +517,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
-      if (n > 0) ok = ok && warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
-      // the row's sum is both halves'
-      s_half[n & 1][t][half][row] = l;
-      meet();
-      l += s_half[n & 1][t][half ^ 1][row];
+      if (ok && n > 0) ok = warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
       if (!ok && lane == 0) *p.status = VQB_TIMEOUT;
       if (ok) {
         tc_fence_after();
@@ -523,7 +529,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         const int64_t at = (pass.part0 + split) * (static_cast<int64_t>(d.n_tokens) * d.heads) + grow;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           if (n > 0) {
             tc_ld32(orow + c * 32, o);
@@ -532,7 +538,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
-          const int col = half * (D / 2) + c * 32;
+          const int col = c * 32;
           if (live && partial) {
             uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + col);
 #pragma unroll
@@ -548,7 +554,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
           }
           __syncwarp();
         }
-        if (live && half == 0) {
+        if (live) {
           if (partial) p.part_ml[at] = make_float2(m, l);
           else if (p.lse) p.lse[grow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
@@ -565,7 +571,7 @@ template <int D, bool BF16>
 vqb_status launch(const AttnParams& p, const AttnPass& pass, unsigned tiles, const CUtensorMap& km, const CUtensorMap& vm,
                   cudaStream_t s) {
   constexpr size_t smem = tiles_smem<D>();
-  static_assert(smem + 4096 <= 232448, "over the opt-in shared memory of an SM");
+  static_assert(smem <= 232448, "over the opt-in shared memory of an SM");
   if (cudaFuncSetAttribute(attention_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
