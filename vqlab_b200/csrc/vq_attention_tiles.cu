@@ -8,9 +8,11 @@
 // tile of 128 keys.  Roles:
 //   * a TMA warp fills a ring of shared-memory stages with K and V tiles, one
 //     box a page and 64 elements (a lane a page);
-//   * one thread issues the MMAs: S = Q_t K^T (both from shared memory) into
-//     tensor memory, then O_t += P_t V with P_t in tensor memory and V read along
-//     its other dimension;
+//   * one thread issues S = Q_t K^T (both from shared memory) into tensor memory,
+//     another O_t += P_t V with P_t in tensor memory and V read along its other
+//     dimension.  Issuing keeps step with the tensor cores, so one thread for both
+//     left them idle while it went from one barrier to the next (3400 cycles a
+//     key tile);
 //   * four softmax warps a tile, a thread a row: the row's 128 scores into
 //     registers, running maximum and sum, weights as 16-bit numbers to tensor
 //     memory.  O is rescaled in place, by the same thread, only when the maximum
@@ -33,8 +35,8 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-constexpr int kThreads = 320;
-constexpr int kWarpMma = 8, kWarpTma = 9;
+constexpr int kThreads = 352;
+constexpr int kWarpQk = 8, kWarpPv = 9, kWarpTma = 10;
 constexpr int kTmemCols = 512;
 template <int D>
 constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
@@ -247,8 +249,8 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   uint64_t* s_read = s_full + 2;       // [2] they are in registers (four warps)
   uint64_t* p_full = s_read + 2;       // [2] its weights are in tensor memory (four warps)
   uint64_t* o_full = p_full + 2;       // [2] its O has this key tile
-  uint64_t* mma_done = o_full + 2;     // [1] teardown
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* mma_done = o_full + 2;     // [2] teardown: an issuer's MMAs are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // values that every lane has alike are broadcast, so that the MMA warp's operands are uniform
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -261,11 +263,11 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
+      mbar_init(&mma_done[t], 1);
       mbar_init(&s_read[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
     }
-    mbar_init(mma_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -349,87 +351,91 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
     // no copy may still be writing shared memory when the block ends
     if (lane == 0)
       for (int k = max(issued - NS, 0); k < issued; ++k) mbar_drain(&kv_full[k % NS], (k / NS) & 1);
-  } else if (warp == kWarpMma) {
-    // ---------------- the MMAs: the warp waits together, one thread issues
-    constexpr uint32_t qk = idesc_f16<BF16>(kTileKeys, false), pv = idesc_f16<BF16>(D, true);
+  } else if (warp == kWarpQk) {
+    // ---------------- S = Q_t K^T for the two tiles in turn: 16 of D a step
+    constexpr uint32_t idesc = idesc_f16<BF16>(kTileKeys, false);
     const bool issuer = elect_one();
-    const uint32_t q0 = smem_u32(q_s), ring0 = smem_u32(ring);
-    auto wait_kv = [&](int idx) { return warp_wait(&kv_full[idx % NS], (idx / NS) & 1, abort_flag); };
-    // S_t = Q_t K^T: 16 of D a step; 64 are 128 contiguous bytes of each row
-    auto mma_qk = [&](int t, int i) {
-      const uint64_t a = desc128(q0 + t * kQTile, 16), b = desc128(ring0 + ((2 * i) % NS) * kStageBytes<D>, 16);
-      if (issuer) {
+    const uint64_t q0 = desc128(smem_u32(q_s), 16), k0 = desc128(smem_u32(ring), 16);
+    bool ok = true;
+    int st = 0, phase = 0;  // K's stage: every second one
+    for (int i = 0; i < n && ok; ++i) {
+      ok = mbar_wait(&kv_full[st], phase, abort_flag);
+      const uint64_t b = k0 + static_cast<uint32_t>(st) * (kStageBytes<D> >> 4);
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
-          tc_mma_ss(s_col, a + off, b + off, qk, ks > 0);
+      for (int t = 0; t < 2; ++t) {
+        if (t == 1 && active < 2) break;
+        // the score tile is free once the scores before are in registers
+        if (t == 1) ok = ok && mbar_wait(&s_read[0], i & 1, abort_flag);
+        else if (i > 0) ok = ok && mbar_wait(&s_read[active - 1], (i - 1) & 1, abort_flag);
+        tc_fence_after();
+        __syncwarp();
+        if (issuer && ok) {
+          const uint64_t a = q0 + t * (kQTile >> 4);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = ((ks >> 2) * kHalf + (ks & 3) * 32) >> 4;
+            tc_mma_ss(s_col, a + off, b + off, idesc, ks > 0);
+          }
+          tc_commit(&s_full[t]);
+          if (t == active - 1) tc_commit(&kv_empty[st]);
         }
-        tc_commit(&s_full[t]);
       }
-      __syncwarp();
-    };
-    // O_t (+)= P_t V: 16 keys a step, up to the last that is held
-    auto mma_pv = [&](int t, int i) {
+      ok = __all_sync(0xffffffffu, ok);
+      st += 2;
+      if (st >= NS) {
+        st -= NS;
+        phase ^= 1;
+      }
+    }
+    if (issuer) {
+      tc_commit(&mma_done[0]);
+      mbar_drain(&mma_done[0], 0);
+    }
+    __syncwarp();
+  } else if (warp == kWarpPv) {
+    // ---------------- O_t (+)= P_t V: 16 keys a step, up to the last that is held
+    constexpr uint32_t idesc = idesc_f16<BF16>(D, true);
+    const bool issuer = elect_one();
+    const uint64_t v0 = desc128(smem_u32(ring), kHalf);
+    bool ok = true;
+    int st = 1, phase = 0;
+    for (int i = 0; i < n && ok; ++i) {
       const bool own = t0 + i >= tiles0;
       const int held = (own ? w.seg1 : w.seg0) - (own ? t0 + i - tiles0 : t0 + i) * kTileKeys;
-      const uint64_t b = desc128(ring0 + ((2 * i + 1) % NS) * kStageBytes<D>, kHalf);
-      if (issuer) {
-        if (held >= kTileKeys) {
-          tc_mma_ts(o_col(t), p_col(t), b, pv, i > 0);
+      const int steps = (min(held, kTileKeys) + 15) / 16;
+      ok = mbar_wait(&kv_full[st], phase, abort_flag);
+      const uint64_t b = v0 + static_cast<uint32_t>(st) * (kStageBytes<D> >> 4);
 #pragma unroll
-          for (int ks = 1; ks < 8; ++ks) tc_mma_ts(o_col(t), p_col(t) + ks * 8, b + ks * (2048 >> 4), pv, 1);
-        } else {
-          for (int ks = 0; ks < (held + 15) / 16; ++ks)
-            tc_mma_ts(o_col(t), p_col(t) + ks * 8, b + ks * (2048 >> 4), pv, i > 0 || ks > 0);
+      for (int t = 0; t < 2; ++t) {
+        if (t == 1 && active < 2) break;
+        ok = ok && mbar_wait(&p_full[t], i & 1, abort_flag);
+        tc_fence_after();
+        __syncwarp();
+        if (issuer && ok) {
+          if (steps == 8) {
+            tc_mma_ts(o_col(t), p_col(t), b, idesc, i > 0);
+#pragma unroll
+            for (int ks = 1; ks < 8; ++ks) tc_mma_ts(o_col(t), p_col(t) + ks * 8, b + ks * (2048 >> 4), idesc, 1);
+          } else {
+            for (int ks = 0; ks < steps; ++ks)
+              tc_mma_ts(o_col(t), p_col(t) + ks * 8, b + ks * (2048 >> 4), idesc, i > 0 || ks > 0);
+          }
+          tc_commit(&o_full[t]);
+          if (t == active - 1) tc_commit(&kv_empty[st]);
         }
-        tc_commit(&o_full[t]);
       }
-      __syncwarp();
-    };
-    auto release = [&](int idx) {
-      if (issuer) tc_commit(&kv_empty[idx % NS]);
-      __syncwarp();
-    };
-    // Q0 K'^T, P1 V, Q1 K'^T, P0 V in turn: a tile's scores are computed while its
-    // softmax warps still work on the weights of the key tile before
-    auto wait_bar = [&](uint64_t* bar, int i) {
-      const bool r = warp_wait(bar, i & 1, abort_flag);
-      tc_fence_after();
-      return r;
-    };
-    const int last = active - 1;
-    bool ok = n > 0 && wait_kv(0);
-    if (ok) {
-      tc_fence_after();
-      mma_qk(0, 0);
+      ok = __all_sync(0xffffffffu, ok);
+      st += 2;
+      if (st >= NS) {
+        st -= NS;
+        phase ^= 1;
+      }
     }
-    for (int i = 0; i < n && ok; ++i) {
-      if (active > 1) {
-        if (!(ok = wait_bar(&s_read[0], i))) break;
-        mma_qk(1, i);
-      }
-      release(2 * i);
-      if (active > 1 && i > 0) {
-        if (!(ok = wait_bar(&p_full[1], i - 1))) break;
-        mma_pv(1, i - 1);
-        release(2 * i - 1);
-      }
-      if (i + 1 < n) {
-        if (!(ok = wait_kv(2 * i + 2) && wait_bar(&s_read[last], i))) break;
-        mma_qk(0, i + 1);
-      }
-      if (!(ok = wait_kv(2 * i + 1) && wait_bar(&p_full[0], i))) break;
-      mma_pv(0, i);
-      if (active == 1) release(2 * i + 1);
+    if (issuer) {
+      tc_commit(&mma_done[1]);
+      mbar_drain(&mma_done[1], 0);
     }
-    if (ok && active > 1 && (ok = wait_bar(&p_full[1], n - 1))) mma_pv(1, n - 1);
-    if (n > 0) {
-      if (issuer) {
-        tc_commit(mma_done);
-        mbar_drain(mma_done, 0);
-      }
-      __syncwarp();
-    }
+    __syncwarp();
   } else {
     // ---------------- softmax: a thread a row
     const int t = warp >> 2;
