@@ -28,6 +28,8 @@
 //
 // Every wait is bounded (2 s): on expiry the block records VQB_TIMEOUT, waits for
 // its copies and MMAs in flight, frees its tensor memory and returns.
+#include <type_traits>
+
 #include "vq_attention.cuh"
 
 namespace vqb {
@@ -38,6 +40,7 @@ constexpr int kTileKeys = 128;
 constexpr int kThreads = 352;
 constexpr int kWarpQk = 8, kWarpPv = 9, kWarpTma = 10;
 constexpr int kTmemCols = 512;
+constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial
 template <int D>
 constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
 template <int D>
@@ -121,12 +124,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// the largest, NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-
 // The largest of 128 scores.
 __device__ __forceinline__ float max128(const float* s) {
   float t[4];
@@ -137,17 +140,46 @@ __device__ __forceinline__ float max128(const float* s) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) t[k] = max3(t[k], s[32 * k + e], s[32 * k + e + 1]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], s[32 * k + 31]);
-  return fmaxf(max3(t[0], t[1], t[2]), t[3]);
+  for (int k = 0; k < 4; ++k) t[k] = max3(t[k], s[32 * k + 31], s[32 * k + 31]);
+  return max3(max3(t[0], t[1], t[2]), t[3], t[3]);
 }
-// Weights 2^(score * scale - base) of 32 scores as 16-bit numbers; returns their sum.
-template <bool BF16>
+
+// 2^x of two numbers on the FMA pipe: x = n + f with n the nearest integer (adding
+// 1.5 * 2^23 leaves n in the sum's low bits), 2^f for f in [-1/2, 1/2] by a
+// polynomial of degree 4 (Remez, relative error 2^-18.5, below the weights' 16
+// bits), n added to the exponent.  x below -126 gives about 2^-126.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
+  float2 x = unpair(x2);
+  x2 = pair(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+  const uint64_t magic = pair(12582912.0f, 12582912.0f), unmagic = pair(-12582912.0f, -12582912.0f);
+  const uint64_t t = add2(x2, magic);
+  const uint64_t f = fma2(add2(t, unmagic), pair(-1.0f, -1.0f), x2);
+  uint64_t r = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
+  r = fma2(r, f, pair(0.240247443318367f, 0.240247443318367f));
+  r = fma2(r, f, pair(0.6931217908859253f, 0.6931217908859253f));
+  r = fma2(r, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  const float2 y = unpair(r), k = unpair(t);
+  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(k.x) << 23)),
+                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(k.y) << 23)));
+}
+
+// Weights 2^(score * scale - base) of 32 scores as 16-bit numbers; returns their
+// sum.  EVERY > 0: every EVERY-th pair on the FMA pipe, which is otherwise little
+// used, since the special function unit's 16 exponentials a cycle bound a tile as
+// much as its MMAs do.
+template <bool BF16, int EVERY>
 __device__ __forceinline__ float weights32(uint32_t (&pk)[16], const float* s, uint64_t scale2, uint64_t base2) {
   uint64_t sum0 = pair(0.f, 0.f), sum1 = sum0;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    const float2 x = unpair(fma2(pair(s[2 * e], s[2 * e + 1]), scale2, base2));
-    const float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+    const uint64_t x2 = fma2(pair(s[2 * e], s[2 * e + 1]), scale2, base2);
+    float2 w;
+    if (EVERY > 0 && e % (EVERY > 0 ? EVERY : 1) == EVERY - 1) {
+      w = exp2_poly(x2);
+    } else {
+      const float2 x = unpair(x2);
+      w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+    }
     if (e & 1) sum1 = add2(sum1, pair(w.x, w.y));
     else sum0 = add2(sum0, pair(w.x, w.y));
     pk[e] = pack16<BF16>(w.x, w.y);
@@ -271,40 +303,43 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncthreads();
   pdl_wait();
   clear_status(p, pass);
   pdl_trigger();
   TileWork w;
   if (!find_work(p, pass, blockIdx.x / d.kv_heads, lane, &w)) return;  // the same for every thread
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   const int kvh = blockIdx.x % d.kv_heads, split = blockIdx.y;
   const int tiles0 = (w.seg0 + kTileKeys - 1) / kTileKeys, all = tiles0 + (w.seg1 + kTileKeys - 1) / kTileKeys;
   const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / pass.splits);
   const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / pass.splits) - t0;
   const int active = w.rows - w.row0 > kTileRows ? 2 : 1;
 
-  // ---- Q into shared memory (128-byte swizzle), rows past the last as zeros
-  for (int i = threadIdx.x; i < active * kTileRows * (D / 8); i += kThreads) {
-    const int row = i / (D / 8), c = i % (D / 8);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    const int g = w.row0 + row;
-    if (g < w.rows) {
-      const int tok = g / p.group;
-      v = *reinterpret_cast<const uint4*>(p.q + (w.rq.q0 + tok) * d.q_token_stride +
-                                          (kvh * p.group + (g - tok * p.group)) * d.q_head_stride + c * 8);
+  uint32_t tmem = 0;
+  if (warp != kWarpTma) {
+    if (warp == kWarpPv) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                   :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp < kWarpQk) {
+      // Q into shared memory (128-byte swizzle), rows past the last as zeros; K's first tiles are on their way meanwhile
+#pragma unroll 4
+      for (int i = threadIdx.x; i < active * kTileRows * (D / 8); i += kWarpQk * 32) {
+        const int row = i / (D / 8), c = i % (D / 8), g = w.row0 + row, gq = min(g, w.rows - 1), tok = gq / p.group;
+        const uint16_t* src = p.q + (w.rq.q0 + tok) * d.q_token_stride + (kvh * p.group + (gq - tok * p.group)) * d.q_head_stride + c * 8;
+        const int tr = row & (kTileRows - 1);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     :: "r"(smem_u32(q_s + (row / kTileRows) * kQTile + (c >> 3) * kHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4))),
+                        "l"(src), "r"(g < w.rows ? 16 : 0) : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    const int tr = row & (kTileRows - 1);
-    *reinterpret_cast<uint4*>(q_s + (row / kTileRows) * kQTile + (c >> 3) * kHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4)) = v;
+    tc_fence_before();
+    asm volatile("barrier.cta.sync 1, %0;" :: "n"(kThreads - 32) : "memory");
+    tc_fence_after();
+    tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   // columns: the scores of either tile, tile t's weights, its output
   const uint32_t s_col = tmem;
   auto p_col = [&](int t) { return tmem + kTileKeys + t * (kTileKeys / 2); };
@@ -464,13 +499,14 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_read[t]);
-        if (__any_sync(0xffffffffu, lim < kTileKeys)) {
+        const bool mask = __any_sync(0xffffffffu, lim < kTileKeys);
+        if (mask) {
 #pragma unroll
           for (int c = 0; c < 128; ++c)
             if (c >= lim) s[c] = -INFINITY;
         }
         const float mx = max128(s) * p.scale_log2;
-        bool fresh = i == 0;  // the weights of the key tile before have met their values
+        bool fresh = i == 0;
         if (__any_sync(0xffffffffu, mx > m + kSlack)) {
           const float mn = fmaxf(m, mx);
           const float f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
@@ -493,19 +529,31 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         }
         const float base = m == -INFINITY ? 0.0f : m;
         const uint64_t base2 = pair(-base, -base);
-        uint32_t pk0[16], pk1[16];
-        l += weights32<BF16>(pk0, s, scale2, base2);
-        l += weights32<BF16>(pk1, s + 32, scale2, base2);
-        if (!fresh) {
-          if (!(ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag))) break;
-          tc_fence_after();
-        }
-        tc_st16(prow, pk0);
-        tc_st16(prow + 16, pk1);
-        l += weights32<BF16>(pk0, s + 64, scale2, base2);
-        tc_st16(prow + 32, pk0);
-        l += weights32<BF16>(pk1, s + 96, scale2, base2);
-        tc_st16(prow + 48, pk1);
+        // the weights of the key tile before have met their values once its MMAs are done
+        auto weights = [&](auto every) {
+          constexpr int kEvery = decltype(every)::value;
+          uint32_t pk0[16], pk1[16];
+          l += weights32<BF16, kEvery>(pk0, s, scale2, base2);
+          l += weights32<BF16, kEvery>(pk1, s + 32, scale2, base2);
+          if (!fresh) {
+            ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
+            tc_fence_after();
+          }
+          if (ok) {
+            tc_st16(prow, pk0);
+            tc_st16(prow + 16, pk1);
+            l += weights32<BF16, kEvery>(pk0, s + 64, scale2, base2);
+            tc_st16(prow + 32, pk0);
+            l += weights32<BF16, kEvery>(pk1, s + 96, scale2, base2);
+            tc_st16(prow + 48, pk1);
+          }
+        };
+        // masked scores have weight 0, not 2^-126
+        if (mask) weights(std::integral_constant<int, 0>{});
+        else weights(std::integral_constant<int, kPolyEvery>{});
+        if (!ok) break;
+        // NaN or inf among the scores: NaN, also where the polynomial clamped it
+        if (!(mx < INFINITY)) l = __int_as_float(0x7FC00000);
         if (t == 0 && (warp & 3) == 0 && (held & 15)) {
           // what lies past the last key may be anything: its weight is 0, its value must be finite
           const int st = (2 * i + 1) % NS;
@@ -534,29 +582,49 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         const bool partial = pass.part0 >= 0;
         const int64_t at = (pass.part0 + split) * (static_cast<int64_t>(d.n_tokens) * d.heads) + grow;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        // through shared memory (Q's, which no MMA reads any more), so that a row leaves as whole lines: D 16-bit
+        // numbers, or half of its fp32 ones at a time
+        constexpr int kRowBytes = D * 2, kRowChunks = kRowBytes / 16;
+        unsigned char* stage = q_s + t * kQTile + (warp & 3) * 32 * kRowBytes;
+        unsigned char* mine = partial ? reinterpret_cast<unsigned char*>(p.part_o + at * D)
+                                      : reinterpret_cast<unsigned char*>(p.out + token * d.out_token_stride + head * d.out_head_stride);
+        for (int pass2 = 0; pass2 < (partial ? 2 : 1); ++pass2) {
+          const int cols = partial ? D / 2 : D;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          if (n > 0) {
-            tc_ld32(orow + c * 32, o);
-            tc_wait_ld32(o);
-          } else {
+          for (int c = 0; c < cols / 32; ++c) {
+            uint32_t o[32];
+            if (n > 0) {
+              tc_ld32(orow + pass2 * (D / 2) + c * 32, o);
+              tc_wait_ld32(o);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+            if (partial) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<uint4*>(stage + lane * kRowBytes + (((c * 8 + e) ^ (lane & 7)) << 4)) =
+                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            } else {
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                pk[e] = pack16<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint4*>(stage + lane * kRowBytes + (((c * 4 + e) ^ (lane & 7)) << 4)) =
+                    make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+            }
+            __syncwarp();
           }
-          const int col = c * 32;
-          if (live && partial) {
-            uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + col);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-          } else if (live) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              pk[e] = pack16<BF16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-            uint4* dst = reinterpret_cast<uint4*>(p.out + token * d.out_token_stride + head * d.out_head_stride + col);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+          const int nlive = min(max(w.rows - (g - lane), 0), 32);  // rows of the warp that exist
+#pragma unroll 4
+          for (int r = 0; r < 32; r += 32 / kRowChunks) {
+            const int rr = r + lane / kRowChunks, c = lane % kRowChunks;
+            const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rr);
+            if (rr < nlive)
+              *reinterpret_cast<uint4*>(reinterpret_cast<unsigned char*>(to) + pass2 * kRowBytes + c * 16) =
+                  *reinterpret_cast<const uint4*>(stage + rr * kRowBytes + ((c ^ (rr & 7)) << 4));
           }
           __syncwarp();
         }
@@ -569,7 +637,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0)
+  if (warp == kWarpPv)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(kTmemCols) : "memory");
 }
 
