@@ -123,6 +123,7 @@ class VQBError(RuntimeError):
 
 _lock = threading.Lock()
 _lib = None
+_native = None
 
 
 def _bind(L):
@@ -214,6 +215,28 @@ def lib():
             except OSError as e:  # no silent fallback: the native path is the product
                 raise RuntimeError(f"libvqb200.so could not be loaded from {LIB_PATH}: {e}") from e
     return _lib
+
+
+def native():
+    """The extension module of the attention calls (csrc/attention_binding.cpp),
+    bound to this library's entry points; built first if it is missing."""
+    global _native
+    if _native is None:
+        L = lib()
+        with _lock:
+            if _native is None:
+                from . import build as _build
+                if not _build.NATIVE.exists():
+                    _build.build_native()
+                try:
+                    from . import _native as m
+                except ImportError as e:  # no silent fallback here either
+                    raise RuntimeError(f"{_build.NATIVE} could not be loaded: {e}") from e
+                addr = lambda f: ctypes.cast(f, ctypes.c_void_p).value  # noqa: E731
+                m.bind(addr(L.vqb_paged_tables), addr(L.vqb_rotary_append),
+                       addr(L.vqb_prefix_attention_workspace_size), addr(L.vqb_prefix_attention))
+                _native = m
+    return _native
 
 
 def status_string(st: int) -> str:

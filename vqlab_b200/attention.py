@@ -2,7 +2,8 @@
 positions and attention, between the q/k/v projections and the output projection.
 
 Three library calls (include/vqb.h), one launch chain each, all on the current
-stream with no host synchronisation:
+stream with no host synchronisation (their arguments are checked and their
+outputs allocated in csrc/attention_binding.cpp):
 
   paged_tables      the step's block tables, lengths and slot map, built on the
                     device from the requests' lengths (vqb_paged_tables)
@@ -20,7 +21,6 @@ Serving only: no gradients.  CUDA tensors only; fp16 and bf16.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import NamedTuple
 
@@ -29,39 +29,12 @@ import torch
 from . import _lib
 from .vq_dense import VQLinear
 
-_HALF = {torch.float16: _lib.VQB_F16, torch.bfloat16: _lib.VQB_BF16}
+_HALF = (torch.float16, torch.bfloat16)
 
 
 def _need(cond: bool, what: str) -> None:
     if not cond:
         raise ValueError(what)
-
-
-def _ints(t: torch.Tensor, name: str, device, shape=None, dtype=torch.int32) -> None:
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == device and t.is_contiguous()
-            and (shape is None or t.shape == shape)):
-        raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor on {device}"
-                         + (f" of shape {tuple(shape)}" if shape is not None else ""))
-
-
-def _heads(t: torch.Tensor, name: str, dtype, device, shape) -> torch.Tensor:
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == device and t.shape == shape
-            and t.stride(-1) == 1):
-        raise ValueError(f"{name} must be a {str(dtype)[6:]} tensor on {device} of shape {tuple(shape)} with "
-                         "contiguous heads")
-    return t
-
-
-def _query(q: torch.Tensor, name: str = "q"):
-    """(N, heads, D, device, dtype) of a tensor of heads."""
-    if not (isinstance(q, torch.Tensor) and q.dtype in _HALF and q.is_cuda and q.dim() == 3 and q.stride(-1) == 1):
-        raise ValueError(f"{name} must be a CUDA tensor [N, heads, D] with contiguous heads, fp16 or bf16")
-    return *q.shape, q.device, q.dtype
-
-
-def _stream(device) -> int:
-    # the raw handle: building a Stream object costs as much as a small call's launch
-    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class PagedTables(NamedTuple):
@@ -86,31 +59,11 @@ def paged_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     and state; otherwise they are left as they are and new tensors returned
     (state[3] counts the call's blocks meanwhile and is 0 again after it).
     max_tokens must cover the new tokens; further places are padding."""
-    _need(isinstance(block_table, torch.Tensor) and block_table.is_cuda and block_table.dim() == 2,
-          "block_table must be a CUDA tensor [R, W]")
-    dev = block_table.device
-    R, W = block_table.shape
-    _ints(block_table, "block_table", dev)
-    _ints(context_lens, "context_lens", dev, (R,))
-    _ints(new_lens, "new_lens", dev, (R,))
-    _ints(free_pages, "free_pages", dev)
-    _need(free_pages.dim() == 1, "free_pages must be a ring [F]")
-    _ints(state, "state", dev, (4,), torch.int64)
-    F, T = free_pages.numel(), int(max_tokens)
-    _need(F > 0 and W > 0 and T >= 0 and page_size > 0, "paged_tables: empty ring or table, or a bad size")
-    if inplace:
-        table, ring, st, lens = block_table, free_pages, state, context_lens
-        flat = block_table.new_empty(R + 1 + 3 * T)
-        cu, s, p, q = flat.split((R + 1, T, T, T))
-    else:
-        table, st = block_table.new_empty((R, W)), state.new_empty(4)
-        ring, lens, cu, s, p, q = block_table.new_empty(F + R + R + 1 + 3 * T).split((F, R, R + 1, T, T, T))
-    d = _lib.PagedDesc(R, W, int(page_size), F, T, int(position_offset))
-    _lib.check(_lib.lib().vqb_paged_tables(
-        ctypes.byref(d), context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(),
-        state.data_ptr(), table.data_ptr(), ring.data_ptr(), st.data_ptr(), lens.data_ptr(), cu.data_ptr(),
-        s.data_ptr(), p.data_ptr(), q.data_ptr(), _stream(dev)), "vqb_paged_tables")
-    return PagedTables(table, lens, cu, s, p, q, ring, st)
+    got = (_lib._native or _lib.native()).paged_tables(context_lens, new_lens, block_table, free_pages, state, page_size,
+                                                       max_tokens, position_offset, inplace)
+    if type(got) is int:
+        _lib.check(got, "vqb_paged_tables")
+    return PagedTables._make(got)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
@@ -155,45 +108,23 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     return the rotated q (in `out`, which may be q).  positions and slots may be
     longer than N (a step's padding).  The tensors may be slices of one fused
     projection: any strides with contiguous heads."""
-    N, H, D, dev, dt = _query(q)
-    _need(isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4, "k_cache must be [pages, kv_heads, page_size, D]")
-    pages, KH, page, _ = k_cache.shape
-    pool = (pages, KH, page, D)
-    _heads(k, "k", dt, dev, (N, KH, D))
-    _heads(v, "v", dt, dev, (N, KH, D))
-    _heads(k_cache, "k_cache", dt, dev, pool)
-    _heads(v_cache, "v_cache", dt, dev, pool)
-    _ints(freq, "freq", dev, None, torch.int64)
-    _ints(positions, "positions", dev)
-    _ints(slots, "slots", dev)
-    _need(positions.numel() >= N and slots.numel() >= N, "positions and slots must cover the tokens")
-    _need(2 * freq.numel() <= D, "freq holds more pairs than a head has")
-    out = q.new_empty((N, H, D)) if out is None else _heads(out, "out", dt, dev, (N, H, D))
-    d = _lib.RotaryDesc(N, H, KH, D, 2 * freq.numel(), int(interleaved), page, pages, float(amplitude),
-                        *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2],
-                        *k_cache.stride()[:3], *v_cache.stride()[:3])
-    _lib.check(_lib.lib().vqb_rotary_append(
-        ctypes.byref(d), _HALF[dt], q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), freq.data_ptr(),
-        slots.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _stream(dev)),
-        "vqb_rotary_append")
-    return out
+    if k is None:
+        raise ValueError("k must be a tensor (rotary() rotates one tensor alone)")
+    got = (_lib._native or _lib.native()).rotary_append(q, k, v, positions, freq, k_cache, v_cache, slots, interleaved,
+                                                        amplitude, out)
+    if type(got) is int:
+        _lib.check(got, "vqb_rotary_append")
+    return got
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, *, interleaved: bool = False,
            amplitude: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate x [N, heads, D] alone (vqb_rotary_append without a cache)."""
-    N, H, D, dev, dt = _query(x, "x")
-    _ints(freq, "freq", dev, None, torch.int64)
-    _ints(positions, "positions", dev)
-    _need(positions.numel() >= N, "positions must cover the tokens")
-    _need(2 * freq.numel() <= D, "freq holds more pairs than a head has")
-    out = x.new_empty((N, H, D)) if out is None else _heads(out, "out", dt, dev, (N, H, D))
-    d = _lib.RotaryDesc(N, H, 0, D, 2 * freq.numel(), int(interleaved), 0, 0, float(amplitude),
-                        *x.stride()[:2], 0, 0, 0, 0, *out.stride()[:2], 0, 0, 0, 0, 0, 0)
-    _lib.check(_lib.lib().vqb_rotary_append(
-        ctypes.byref(d), _HALF[dt], x.data_ptr(), None, None, positions.data_ptr(), freq.data_ptr(), None,
-        out.data_ptr(), None, None, _stream(dev)), "vqb_rotary_append")
-    return out
+    got = (_lib._native or _lib.native()).rotary_append(x, None, None, positions, freq, None, None, None, interleaved,
+                                                        amplitude, out)
+    if type(got) is int:
+        _lib.check(got, "vqb_rotary_append")
+    return got
 
 
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -210,40 +141,12 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     requests' lengths, which stay on the device.  scale defaults to D ** -0.5.
     Returns [N, heads, D], and with return_lse the fp32 log-sum-exp [N, heads]
     of the scaled scores; rows past cu_q[-1] are not written."""
-    N, H, D, dev, dt = _query(q)
-    _need(isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4, "k_cache must be [pages, kv_heads, page_size, D]")
-    pages, KH, page, _ = k_cache.shape
-    pool = (pages, KH, page, D)
-    _need(KH > 0 and H % KH == 0, "heads must be a multiple of kv_heads")
-    _heads(k_cache, "k_cache", dt, dev, pool)
-    _heads(v_cache, "v_cache", dt, dev, pool)
-    _ints(kv_lens, "kv_lens", dev)
-    R = kv_lens.numel()
-    _ints(cu_q, "cu_q", dev, (R + 1,))
-    _ints(block_table, "block_table", dev)
-    _need(block_table.dim() == 2 and block_table.shape[0] == R, "block_table must be [R, W]")
-    if prefix_len:
-        _need(prefix_pages is not None, "prefix_len needs prefix_pages")
-        _ints(prefix_pages, "prefix_pages", dev)
-        _need(prefix_pages.numel() * page >= prefix_len, "prefix_pages must cover prefix_len")
-    out = q.new_empty((N, H, D)) if out is None else _heads(out, "out", dt, dev, (N, H, D))
-    lse = q.new_empty((N, H), dtype=torch.float32) if return_lse else None
-    d = _lib.AttentionDesc(R, N, H, KH, D, page, pages, block_table.shape[1], int(max_q_len), int(max_kv_len),
-                           int(prefix_len), int(causal), D ** -0.5 if scale is None else float(scale),
-                           *q.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3])
-    L = _lib.lib()
-    nbytes = L.vqb_prefix_attention_workspace_size(ctypes.byref(d))
-    if workspace is None:
-        workspace = q.new_empty(nbytes or 256, dtype=torch.uint8)
-    else:
-        if not (workspace.dtype == torch.uint8 and workspace.device == dev and workspace.numel() >= nbytes):
-            raise ValueError(f"workspace must be a uint8 CUDA tensor of >= {nbytes} bytes")
-    _lib.check(L.vqb_prefix_attention(
-        ctypes.byref(d), _HALF[dt], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-        kv_lens.data_ptr(), cu_q.data_ptr(), prefix_pages.data_ptr() if prefix_len else None, out.data_ptr(),
-        lse.data_ptr() if return_lse else None, workspace.data_ptr(), workspace.numel(), _stream(dev)),
-        "vqb_prefix_attention")
-    return (out, lse) if return_lse else out
+    got = (_lib._native or _lib.native()).prefix_attention(q, k_cache, v_cache, block_table, kv_lens, cu_q, max_q_len,
+                                                           max_kv_len, prefix_pages, prefix_len, scale, causal, out,
+                                                           return_lse, workspace)
+    if type(got) is int:
+        _lib.check(got, "vqb_prefix_attention")
+    return got
 
 
 class PagedKVCache:

@@ -6,6 +6,9 @@
 Each csrc/*.cu is compiled to an object under vqlab_b200/_build/ (in
 parallel), then linked into vqlab_b200/libvqb200.so with the static CUDA
 runtime, so the library carries no torch or libcudart version dependency.
+csrc/attention_binding.cpp becomes the Python extension module _native, built
+against the installed torch (it hands the library's entry points to the
+attention calls; the library does not depend on it).
 """
 from __future__ import annotations
 
@@ -16,12 +19,16 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libvqb200.so"
+
+BINDING = CSRC / "attention_binding.cpp"
+NATIVE = PKG / ("_native" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3",
@@ -50,6 +57,31 @@ def _stale(target: pathlib.Path, deps) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_native(force: bool = False, verbose: bool = False) -> pathlib.Path:
+    """The Python extension module of the attention calls."""
+    if not (force or _stale(NATIVE, [BINDING, ROOT / "include" / "vqb.h"])):
+        return NATIVE
+    import torch
+
+    tdir = pathlib.Path(torch.__file__).parent
+    cuda = pathlib.Path(nvcc()).resolve().parent.parent
+    tmp = NATIVE.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-shared", "-fPIC", "-O2", "-std=c++17",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include")]
+    for inc in ("include", "include/torch/csrc/api/include"):
+        cmd += ["-isystem", str(tdir / inc)]
+    cmd += [str(BINDING), "-o", str(tmp), "-L", str(tdir / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+            "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compiling {BINDING.name} failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, NATIVE)
+    return NATIVE
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> pathlib.Path:
     BUILD.mkdir(exist_ok=True)
     srcs = _sources()
@@ -70,8 +102,10 @@ def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> 
                 sys.stderr.write(r.stderr)
         return obj
 
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        native = ex.submit(build_native, force, verbose)
         objs = list(ex.map(compile_one, srcs))
+        native.result()
     if force or _stale(LIB, objs):
         tmp = LIB.with_suffix(".so.tmp")
         cmd = [cc] + ARCH + ["-shared", "-cudart", "static", "-o", str(tmp)] + [str(o) for o in objs]
