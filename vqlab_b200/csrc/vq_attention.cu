@@ -20,7 +20,8 @@ struct AttnPlan {
   AttnPass own;
   bool decode;         // the own pass runs the decode kernel
   unsigned shared_tiles, own_tiles;
-  int parts;           // partial results; 0: the own pass writes out
+  int parts;           // partial results in the workspace
+  bool join;           // a join kernel follows (else the own pass writes out)
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -57,33 +58,34 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   if (joint) {
     a.shared_tiles = static_cast<unsigned>(ceil_div(rows, 256));
     a.shared = AttnPass{1, 0, pick_splits(static_cast<int64_t>(a.shared_tiles) * d.kv_heads, ceil_div(d.prefix_len, 128),
-                                          sms, row_cost, true), 0, 0, 1};
+                                          sms, row_cost, true), 0, 1, 0, 1};
   }
   const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
   a.own.prefix = !joint && d.prefix_len > 0;
   if (a.decode) {
-    // a block streams 256 keys or more; about two rounds of two blocks an SM
+    // About five rounds of three blocks an SM, so that ragged lengths even out, each
+    // with 256 keys or more: up to 8 blocks a (request, head) in a cluster, and
+    // several clusters only where 8 would leave SMs idle.
     const int64_t blocks = static_cast<int64_t>(d.n_requests) * d.kv_heads;
-    int64_t s = ceil_div(4 * sms, blocks);
+    int64_t s = ceil_div(15 * sms, blocks);
     if (s > ceil_div(keys, 256)) s = ceil_div(keys, 256);
-    if (s > 64) s = 64;
-    if (s < 1) s = 1;
-    a.own.chunk = static_cast<int>(ceil_div(ceil_div(keys, s), 64) * 64);
-    if (a.own.prefix) a.own.chunk += 64;  // the prefix and the own keys start groups of their own
-    if (a.own.chunk < 64) a.own.chunk = 64;
-    a.own.splits = static_cast<int>(s);
+    a.own.cluster = 1;
+    while (a.own.cluster < 8 && a.own.cluster * 2 <= s) a.own.cluster *= 2;
+    a.own.splits = 1;
+    if (blocks * 8 < sms && s > 8) {
+      s = ceil_div(2 * sms, blocks * 8) < s / 8 ? ceil_div(2 * sms, blocks * 8) : s / 8;
+      a.own.splits = static_cast<int>(s < 16 ? s : 16);
+    }
   } else {
     a.own_tiles = static_cast<unsigned>(rows / 256 + d.n_requests);
     const int64_t blocks = (rows / 256 > d.n_requests ? rows / 256 : d.n_requests) * d.kv_heads;
     a.own.splits = pick_splits(blocks, ceil_div(keys, 128), sms, row_cost, joint);
   }
   a.own.first = a.shared.splits == 0;
-  a.parts = a.shared.splits + a.own.splits;
-  a.own.part0 = a.shared.splits;
-  if (a.parts == 1) {
-    a.own.part0 = -1;
-    a.parts = 0;
-  }
+  a.join = a.own.splits > 1 || (!a.decode && a.shared.splits > 0);
+  a.own.part0 = a.join ? a.shared.splits : -1;
+  a.own.joins = a.join ? 0 : a.shared.splits;
+  a.parts = a.shared.splits + (a.join ? a.own.splits : 0);
   return a;
 }
 
@@ -223,7 +225,7 @@ extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_d
   }
   st = a.decode ? launch_attention_decode(p, a.own, bf, s) : launch_attention_tiles(p, a.own, bf, a.own_tiles, s);
   if (st != VQB_OK) return st;
-  if (a.parts > 0) st = launch_join(p, a.parts, bf, s);
+  if (a.join) st = launch_join(p, a.parts, bf, s);
   timer_after(s);
   return st;
 }

@@ -34,8 +34,9 @@ struct AttnPass {
   int joint;     // rows of all requests together, over the shared prefix alone
   int prefix;    // (not joint) the request's keys begin with the shared prefix
   int splits;
-  int part0;     // first partial result of the pass; -1: the pass writes out itself
-  int chunk;     // decode kernel: keys of a split
+  int part0;     // first partial result of the pass, one a split; -1: the pass writes out itself
+  int cluster;   // decode kernel: blocks of a cluster, which share a split's keys
+  int joins;     // decode kernel: partial results 0 .. joins - 1 to join with its own
   int first;     // the call's first pass: its first block clears the status block
 };
 

@@ -1,16 +1,23 @@
 // Attention of requests with few query rows (tokens x heads of a group <= 16)
 // over their own keys: one pass over the cache, bound by its bytes.
 //
-// A block takes (request, key/value head, a run of keys).  Its four warps are
-// independent: each streams every fourth group of 16 keys through its own ring
-// of shared-memory stages (four 2 KB TMA boxes a stage at D = 128; the warp's
-// first lane refills a stage as soon as the warp has read it), with its own
-// running maximum and sum.  A warp computes S = Q K^T and O += P V with
-// m16n8k16 MMAs: Q and O stay in registers, P goes from the accumulator's
-// layout straight into the next MMA's operand.  These MMAs run far below the
-// tensor cores' rate, but a group's 8 KB take 350 cycles of an SM's share of
-// memory bandwidth and 64 of its MMA pipe.  At the end the four warps' results
-// are joined in shared memory.
+// A cluster of blocks takes (request, key/value head) and splits its keys evenly.
+// A block's four warps are independent: each streams every fourth group of 16
+// keys of the block's run through its own ring of shared-memory stages (four 2 KB
+// TMA boxes a stage at D = 128; the warp's first lane refills a stage as soon as
+// the warp has read it), with its own running maximum and sum.  A warp computes
+// S = Q K^T and O += P V with m16n8k16 MMAs: Q and O stay in registers, P goes from
+// the accumulator's layout straight into the next MMA's operand.  These MMAs run
+// far below the tensor cores' rate, but a group's 8 KB take 350 cycles of an SM's
+// share of memory bandwidth and 64 of its MMA pipe.
+//
+// The results are joined without leaving the kernel: the four warps' in shared
+// memory, then the cluster's over distributed shared memory (each block joins its
+// share of the rows), then, when the batch has a shared prefix, with the partial
+// results of the pass over the prefix.  That pass is the kernel before this one on
+// the stream; this one starts as its blocks end and waits for it only here.  Only
+// where eight blocks for a (request, head) would leave most SMs idle do several
+// clusters share it, and a join kernel follows.
 #include "vq_attention.cuh"
 
 namespace vqb {
@@ -19,11 +26,59 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;  // keys of a stage
 template <int D>
-constexpr int kStages = D == 128 ? 3 : 6;  // 24 KB a warp, 96 KB a block, two blocks an SM
+constexpr int kStages = D == 128 ? 2 : 4;  // 16 KB a warp, 64 KB a block, three blocks an SM
 template <int D>
 constexpr int kHalfBytes = kUnit * D * 2;  // K or V of a stage
 template <int D>
-constexpr size_t decode_smem() { return 1024 + size_t(kWarps) * kStages<D> * 2 * kHalfBytes<D>; }
+constexpr size_t kRingBytes = size_t(kStages<D>) * 2 * kHalfBytes<D>;  // of a warp; at the end fp32 [16][D]
+template <int D>
+constexpr size_t decode_smem() { return 1024 + kWarps * kRingBytes<D>; }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+// every thread of every block of the cluster, always the same number of times
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 ld_remote4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 ld_remote2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+
+// A running join of partial results (m, l, four elements of O).
+struct Joined {
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float pm, float pl, float4 po) {
+    const float mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.0f : mn;
+    const float f = exp2_fast(m - base), g = exp2_fast(pm - base);
+    m = mn;
+    l = l * f + pl * g;
+    o.x = o.x * f + po.x * g;
+    o.y = o.y * f + po.y * g;
+    o.z = o.z * f + po.z * g;
+    o.w = o.w * f + po.w * g;
+  }
+};
 
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -46,12 +101,13 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+__global__ void __launch_bounds__(kWarps * 32, 3)
 attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t s_full[kWarps][kStages<D>];
   __shared__ float s_m[kWarps][16], s_l[kWarps][16];
+  __shared__ float2 s_ml[16];  // the block's own
   __shared__ int s_abort;
   constexpr int NS = kStages<D>;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -64,21 +120,31 @@ attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUt
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  pdl_wait();
+  // With a pass over the prefix before this kernel, that pass's blocks have all
+  // waited for what came before them by the time this one may start, and only its
+  // results have to be waited for, below.
+  if (pass.first) pdl_wait();
+  pdl_trigger();
   clear_status(p, pass);
 
-  const int kvh = blockIdx.y, r = blockIdx.z, split = blockIdx.x;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int kvh = blockIdx.y, r = blockIdx.z;
+  const int cluster = blockIdx.x / ranks;
   const RequestRows rq = request_rows(p, r);
   const int nrows = min(rq.nq * p.group, 16);
-  if (nrows == 0) return;
+  if (nrows == 0) {  // the same for the whole cluster
+    if (!pass.first) pdl_wait();  // whoever waits for this kernel also waits for the pass before it
+    return;
+  }
   const int seg0 = pass.prefix ? d.prefix_len : 0;
   const int seg1 = visible(p, rq, rq.nq - 1);
   const int tiles0 = (seg0 + kUnit - 1) / kUnit, tiles = tiles0 + (seg1 + kUnit - 1) / kUnit;
-  const int per = pass.chunk / kUnit;
-  const int u0 = min(split * per, tiles), u1 = min(u0 + per, tiles);
+  const int split = cluster * ranks + rank, splits = gridDim.x;
+  const int u0 = static_cast<int>(static_cast<int64_t>(tiles) * split / splits);
+  const int u1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / splits);
   // this warp's groups: u0 + warp, then every fourth
   const int n = u1 - u0 > warp ? (u1 - u0 - warp + kWarps - 1) / kWarps : 0;
-  unsigned char* ring = smem + static_cast<size_t>(warp) * NS * 2 * kHalfBytes<D>;
+  unsigned char* ring = smem + warp * kRingBytes<D>;
 
   auto page_of = [&](int k) -> int {  // page of the warp's k-th group
     if (k >= n) return d.num_pages;
@@ -127,7 +193,6 @@ attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUt
     }
   }
   const int vis0 = visible(p, rq, min(row0 / p.group, rq.nq - 1)), vis1 = visible(p, rq, min(row1 / p.group, rq.nq - 1));
-  pdl_trigger();
 
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, o[D / 8][4];
 #pragma unroll
@@ -250,40 +315,53 @@ attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUt
   }
   __syncthreads();
   constexpr int kPer = D / 4;  // threads of a row, four elements each
-  constexpr size_t kRing = size_t(NS) * 2 * kHalfBytes<D> / sizeof(float);
-  const float* rings = reinterpret_cast<const float*>(smem);
+  constexpr size_t kRing = kRingBytes<D> / sizeof(float);
+  float* rings = reinterpret_cast<float*>(smem);
   for (int i = threadIdx.x; i < nrows * kPer; i += kWarps * 32) {
     const int row = i / kPer, e = (i % kPer) * 4;
-    float m = s_m[0][row];
+    Joined j;
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w][row]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2_fast(s_m[w][row] - base);
-      const float4 x = *reinterpret_cast<const float4*>(rings + w * kRing + row * D + e);
-      l += s_l[w][row] * f;
-      a.x += x.x * f;
-      a.y += x.y * f;
-      a.z += x.z * f;
-      a.w += x.w * f;
+    for (int w = 0; w < kWarps; ++w)
+      j.add(s_m[w][row], s_l[w][row], *reinterpret_cast<const float4*>(rings + w * kRing + row * D + e));
+    *reinterpret_cast<float4*>(rings + row * D + e) = j.o;  // this thread alone reads these elements
+    if (e == 0) s_ml[row] = make_float2(j.m, j.l);
+  }
+  if (ranks > 1) cluster_sync();
+  else __syncthreads();
+  const bool partial = pass.part0 >= 0;
+  if (!pass.first && !partial) pdl_wait();  // the prefix's partial results
+  // ---- rows dealt over the cluster's blocks
+  const int64_t all_rows = static_cast<int64_t>(d.n_tokens) * d.heads;
+  for (int i = threadIdx.x; i < ((nrows - static_cast<int>(rank) + static_cast<int>(ranks) - 1) / static_cast<int>(ranks)) * kPer;
+       i += kWarps * 32) {
+    const int row = (i / kPer) * ranks + rank, e = (i % kPer) * 4;
+    Joined j;
+    for (uint32_t c = 0; c < ranks; ++c) {
+      const float2 ml = ld_remote2(remote(&s_ml[row], c));
+      j.add(ml.x, ml.y, ld_remote4(remote(rings + row * D + e, c)));
     }
     const int64_t tok = rq.q0 + row / p.group;
     const int head = kvh * p.group + row % p.group;
     const int64_t grow = tok * d.heads + head;
-    if (pass.part0 >= 0) {
-      const int64_t at = (pass.part0 + split) * (static_cast<int64_t>(d.n_tokens) * d.heads) + grow;
-      *reinterpret_cast<float4*>(p.part_o + at * D + e) = a;
-      if (e == 0) p.part_ml[at] = make_float2(m, l);
+    if (partial) {
+      const int64_t at = (pass.part0 + cluster) * all_rows + grow;
+      *reinterpret_cast<float4*>(p.part_o + at * D + e) = j.o;
+      if (e == 0) p.part_ml[at] = make_float2(j.m, j.l);
     } else {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const uint2 w = make_uint2(pack16<BF16>(a.x * inv, a.y * inv), pack16<BF16>(a.z * inv, a.w * inv));
+#pragma unroll 4
+      for (int i2 = 0; i2 < pass.joins; ++i2) {
+        const int64_t at = i2 * all_rows + grow;
+        const float2 ml = __ldcg(p.part_ml + at);
+        j.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + e)));
+      }
+      const float inv = j.l == 0.0f ? 0.0f : 1.0f / j.l;
+      const uint2 w = make_uint2(pack16<BF16>(j.o.x * inv, j.o.y * inv), pack16<BF16>(j.o.z * inv, j.o.w * inv));
       *reinterpret_cast<uint2*>(p.out + tok * d.out_token_stride + head * d.out_head_stride + e) = w;
-      if (p.lse && e == 0) p.lse[grow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+      if (p.lse && e == 0) p.lse[grow] = j.l == 0.0f ? -INFINITY : (j.m + log2f(j.l)) * kLn2;
     }
   }
+  if (ranks > 1) cluster_sync();  // no block leaves while another reads its memory
+  if (!pass.first && partial) pdl_wait();
 }
 
 template <int D, bool BF16>
@@ -292,9 +370,21 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, const CUtensorMap& 
   if (cudaFuncSetAttribute(attention_decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
-  const dim3 grid(pass.splits, p.d.kv_heads, p.d.n_requests);
-  if (launch_pdl(attention_decode_kernel<D, BF16>, grid, kWarps * 32, smem, s, p, pass, km, vm) != cudaSuccess)
-    return VQB_CUDA_ERROR;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = pass.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pass.splits * pass.cluster, p.d.kv_heads, p.d.n_requests);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, attention_decode_kernel<D, BF16>, p, pass, km, vm) != cudaSuccess) return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
 }
