@@ -63,12 +63,12 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
   a.own.prefix = !joint && d.prefix_len > 0;
   if (a.decode) {
-    // About five rounds of three blocks an SM, so that ragged lengths even out, each
-    // with 256 keys or more: up to 8 blocks a (request, head) in a cluster, and
+    // About two rounds of three blocks an SM, so that ragged lengths even out, each
+    // with 512 keys or more: up to 8 blocks a (request, head) in a cluster, and
     // several clusters only where 8 would leave SMs idle.
     const int64_t blocks = static_cast<int64_t>(d.n_requests) * d.kv_heads;
-    int64_t s = ceil_div(15 * sms, blocks);
-    if (s > ceil_div(keys, 256)) s = ceil_div(keys, 256);
+    int64_t s = ceil_div(6 * sms, blocks);
+    if (s > ceil_div(keys, 512)) s = ceil_div(keys, 512);
     a.own.cluster = 1;
     while (a.own.cluster < 8 && a.own.cluster * 2 <= s) a.own.cluster *= 2;
     a.own.splits = 1;

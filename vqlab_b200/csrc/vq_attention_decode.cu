@@ -26,7 +26,9 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kUnit = 16;  // keys of a stage
 template <int D>
-constexpr int kStages = D == 128 ? 2 : 4;  // 16 KB a warp, 64 KB a block, three blocks an SM
+constexpr int kStages = D == 128 ? 2 : 3;
+template <int D>
+constexpr int kResident = D == 128 ? 3 : 4;  // blocks an SM: of 64 KB and 168 registers, of 48 KB and 128 registers
 template <int D>
 constexpr int kHalfBytes = kUnit * D * 2;  // K or V of a stage
 template <int D>
@@ -101,7 +103,7 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, 3)
+__global__ void __launch_bounds__(kWarps * 32, kResident<D>)
 attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char smem_raw[];
