@@ -19,30 +19,72 @@ struct AttnPlan {
   AttnPass shared;     // splits = 0: no pass over the prefix alone
   AttnPass own;
   bool decode;         // the own pass runs the decode kernel
-  unsigned shared_tiles, own_tiles;
+  int64_t shared_tiles, own_tiles;  // pairs of row tiles (own: an upper bound)
   int parts;           // partial results in the workspace
   bool join;           // a join kernel follows (else the own pass writes out)
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How many splits of `tiles` key tiles (a tile costs one) finish first: rounds
-// of blocks over the SMs times the longest block (its tiles and about three
-// tiles' worth of start and end), and the join's traffic (`row_cost`: partial
-// result of one split, in tiles).
+// Times in microseconds, measured at D = 128: a key tile of a block with two row
+// tiles, with one, and a block's start and end.
+constexpr double kPairTile = 1.5, kOneTile = 1.2, kBlockEnds = 7.0;
+constexpr int kMaxSplits = 64;
+
+// Splits of `tiles` key tiles over the tile kernel's blocks: the fewest rounds of
+// the longest block, and the join's traffic (`row_cost`: a partial result's).
 int pick_splits(int64_t blocks, int64_t tiles, int slots, double row_cost, bool joined_anyway) {
   int best = 1;
   double best_t = 1e30;
-  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+  for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
     const double rounds = static_cast<double>(ceil_div(blocks * s, slots));
-    double t = rounds * (static_cast<double>(ceil_div(tiles, s)) + 3.0);
-    if (s > 1 || joined_anyway) t += row_cost * s + 3.0;
+    double t = rounds * (static_cast<double>(ceil_div(tiles, s)) * kPairTile + kBlockEnds);
+    if (s > 1 || joined_anyway) t += row_cost * s + 4.0;
     if (t < best_t * 0.98) {
       best_t = t;
       best = s;
     }
   }
   return best;
+}
+
+// Splits of the pass over the prefix before a decode pass over the requests' own
+// keys, which takes `alone` us by itself (bound by memory) and needs `other` SM
+// microseconds.  Either it has all SMs first and the decode pass joins the partial
+// results, or it leaves SMs on which the decode pass runs at the same time (one is
+// bound by arithmetic, the other by memory), and a join kernel follows (about 9 us).
+// Measured: 250 requests behind 32768 keys with up to 2000 of their own 306 us in
+// turn, 274 us together (2 splits: 80 blocks); 64 requests behind 16421 keys with up
+// to 500 of their own 52 us in turn, 56 us together.  Returns true for the latter.
+bool pick_shared_splits(AttnPass* a, int64_t full, bool rest, int heads, int64_t tiles, int sms, double row_cost,
+                        double other, double alone) {
+  double best_t = 1e30;
+  bool together = false;
+  for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
+    const int s2 = rest ? static_cast<int>(s * kOneTile / kPairTile + 0.999) : 0;
+    const int64_t n1 = full * s * heads, n2 = static_cast<int64_t>(s2) * heads;
+    const double t1 = full ? kBlockEnds + kPairTile * ceil_div(tiles, s) : 0.0;
+    const double t2 = rest ? kBlockEnds + kOneTile * ceil_div(tiles, s2) : 0.0;
+    const double longest = t1 > t2 ? t1 : t2;
+    for (int mode = 0; mode < 2; ++mode) {
+      double t;
+      if (mode == 0) {
+        t = ceil_div(n1 + n2, sms) * longest + alone + row_cost * s;
+      } else {
+        if (n1 + n2 > sms) continue;  // none left
+        t = (n1 * t1 + n2 * t2 + other) / sms;
+        if (t < longest) t = longest;
+        t += row_cost * (s + 1) + 9.0;
+      }
+      if (t < best_t * 0.98) {
+        best_t = t;
+        a->splits = s;
+        a->rest = s2;
+        together = mode == 1;
+      }
+    }
+  }
+  return together;
 }
 
 AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
@@ -52,39 +94,50 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   const int64_t most = static_cast<int64_t>(d.max_q_len < d.n_tokens ? d.max_q_len : d.n_tokens) * group;
   a.decode = most <= 16;
   // the prefix for all rows at once, unless a request fills tiles by itself
-  const bool joint = d.prefix_len > 0 && d.n_requests > 1 && most <= 256;
-  // a partial result's bytes over the time of a key tile (about 1 us at 4 TB/s)
+  const bool joint = d.prefix_len > 0 && d.n_requests > 1 && most <= kPairRows;
+  // a partial result written and read, at 4 TB/s
   const double row_cost = static_cast<double>(d.n_tokens) * d.heads * d.head_dim * 8.0 / 4.0e6;
-  if (joint) {
-    a.shared_tiles = static_cast<unsigned>(ceil_div(rows, 256));
-    a.shared = AttnPass{1, 0, pick_splits(static_cast<int64_t>(a.shared_tiles) * d.kv_heads, ceil_div(d.prefix_len, 128),
-                                          sms, row_cost, true), 0, 1, 0, 1};
-  }
   const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
+  const int64_t requests_heads = static_cast<int64_t>(d.n_requests) * d.kv_heads;
   a.own.prefix = !joint && d.prefix_len > 0;
   if (a.decode) {
     // About two rounds of three blocks an SM, so that ragged lengths even out, each
     // with 512 keys or more: up to 8 blocks a (request, head) in a cluster, and
     // several clusters only where 8 would leave SMs idle.
-    const int64_t blocks = static_cast<int64_t>(d.n_requests) * d.kv_heads;
-    int64_t s = ceil_div(6 * sms, blocks);
+    int64_t s = ceil_div(6 * sms, requests_heads);
     if (s > ceil_div(keys, 512)) s = ceil_div(keys, 512);
     a.own.cluster = 1;
     while (a.own.cluster < 8 && a.own.cluster * 2 <= s) a.own.cluster *= 2;
     a.own.splits = 1;
-    if (blocks * 8 < sms && s > 8) {
-      s = ceil_div(2 * sms, blocks * 8) < s / 8 ? ceil_div(2 * sms, blocks * 8) : s / 8;
+    if (requests_heads * 8 < sms && s > 8) {
+      s = ceil_div(2 * sms, requests_heads * 8) < s / 8 ? ceil_div(2 * sms, requests_heads * 8) : s / 8;
       a.own.splits = static_cast<int>(s < 16 ? s : 16);
     }
   } else {
-    a.own_tiles = static_cast<unsigned>(rows / 256 + d.n_requests);
-    const int64_t blocks = (rows / 256 > d.n_requests ? rows / 256 : d.n_requests) * d.kv_heads;
+    a.own_tiles = rows / kPairRows + d.n_requests;
+    const int64_t blocks = (rows / kPairRows > d.n_requests ? rows / kPairRows : d.n_requests) * d.kv_heads;
     a.own.splits = pick_splits(blocks, ceil_div(keys, 128), sms, row_cost, joint);
   }
+  bool together = !a.decode;  // the own pass leaves partial results too
+  if (joint) {
+    a.shared.joint = 1;
+    a.shared.first = 1;
+    a.shared_tiles = ceil_div(rows, kPairRows);
+    const bool rest = rows % kPairRows > 0 && rows % kPairRows <= kPairRows / 2;
+    const int64_t tiles = ceil_div(d.prefix_len, 128);
+    if (a.decode) {
+      // an SM's time for the own keys: 100 GB/s and 2 us a block, with lengths that average 0.6 of the largest
+      const double bytes = 0.6 * keys * requests_heads * d.head_dim * 4.0;
+      const double other = bytes / 1.0e5 + 2.0 * requests_heads * a.own.cluster;
+      const double alone = bytes / 6.4e6 > other / sms ? bytes / 6.4e6 : other / sms;
+      together = pick_shared_splits(&a.shared, a.shared_tiles - rest, rest, d.kv_heads, tiles, sms, row_cost, other, alone);
+    } else {
+      a.shared.splits = pick_splits(a.shared_tiles * d.kv_heads, tiles, sms, row_cost, true);
+    }
+  }
   a.own.first = a.shared.splits == 0;
-  a.join = a.own.splits > 1 || (!a.decode && a.shared.splits > 0);
+  a.join = a.own.splits > 1 || (a.shared.splits > 0 && together);
   a.own.part0 = a.join ? a.shared.splits : -1;
-  a.own.joins = a.join ? 0 : a.shared.splits;
   a.parts = a.shared.splits + (a.join ? a.own.splits : 0);
   return a;
 }
@@ -94,10 +147,11 @@ constexpr size_t kStatusBytes = 256;
 size_t part_rows(const vqb_attention_desc& d) { return static_cast<size_t>(d.n_tokens) * d.heads; }
 size_t ml_bytes(const vqb_attention_desc& d, int parts) { return (parts * part_rows(d) * sizeof(float2) + 255) & ~size_t(255); }
 
-// Joins a row's partial results, a warp a row.  Bound: the partial results'
-// bytes, which are in L2 as a rule.
+// Joins a row's partial results, a warp a row: a lane weighs a part, then the
+// parts' elements are read without waiting for one another.  Bound: the partial
+// results' bytes, which are in L2 as a rule.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, int parts) {
+__global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, AttnPass shared, int own_parts) {
   pdl_wait();
   pdl_trigger();
   const vqb_attention_desc& d = p.d;
@@ -108,30 +162,42 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, int p
   const int64_t n = row / d.heads;
   const int h = static_cast<int>(row - n * d.heads);
   if (n >= __ldg(p.cu_q + d.n_requests)) return;
-  float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(p.part_ml + i * rows + row).x);
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float base = m == -INFINITY ? 0.0f : m;
+  const int ns = shared.splits ? shared_parts(shared, d.n_tokens * p.group, n * p.group + h % p.group) : 0;
+  const int parts = ns + own_parts;  // the own pass's follow the `splits` places of the shared one's
   constexpr int kPer = D / 32;
-  float acc[kPer], l = 0.0f;
+  float m = -INFINITY, l = 0.0f, acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
-  for (int i = 0; i < parts; ++i) {
-    const float2 ml = __ldcg(p.part_ml + i * rows + row);
-    if (ml.y == 0.0f) continue;  // nothing seen in that part
-    const float f = exp2_fast(ml.x - base);
-    l += ml.y * f;
-    const float* o = p.part_o + (i * rows + row) * D + lane * kPer;
-    if constexpr (kPer == 4) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(o));
-      acc[0] += v.x * f;
-      acc[1] += v.y * f;
-      acc[2] += v.z * f;
-      acc[3] += v.w * f;
-    } else {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(o));
-      acc[0] += v.x * f;
-      acc[1] += v.y * f;
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    const int i = i0 + lane;
+    const int64_t at = (i < ns ? i : i - ns + shared.splits) * rows + row;
+    const float2 ml = i < parts ? __ldcg(p.part_ml + at) : make_float2(-INFINITY, 0.0f);
+    float top = ml.x;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
+    const float keep = exp2_fast(m - base), w = exp2_fast(ml.x - base);
+    m = mn;
+    float sum = ml.y * w;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = l * keep + sum;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] *= keep;
+    const int here = min(parts - i0, 32);
+#pragma unroll 4
+    for (int k = 0; k < here; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      const float* o = p.part_o + __shfl_sync(0xffffffffu, at, k) * D + lane * kPer;
+      if constexpr (kPer == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(o));
+        acc[0] += v.x * wk;
+        acc[1] += v.y * wk;
+        acc[2] += v.z * wk;
+        acc[3] += v.w * wk;
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(o));
+        acc[0] += v.x * wk;
+        acc[1] += v.y * wk;
+      }
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -141,15 +207,15 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, int p
   if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-vqb_status launch_join(const AttnParams& p, int parts, bool bf, cudaStream_t s) {
+vqb_status launch_join(const AttnParams& p, const AttnPass& shared, int own_parts, bool bf, cudaStream_t s) {
   const unsigned blocks = static_cast<unsigned>((part_rows(p.d) + 7) / 8);
   cudaError_t ce;
   if (p.d.head_dim == 128)
-    ce = bf ? launch_pdl(attention_join_kernel<128, true>, blocks, 256, 0, s, p, parts)
-            : launch_pdl(attention_join_kernel<128, false>, blocks, 256, 0, s, p, parts);
+    ce = bf ? launch_pdl(attention_join_kernel<128, true>, blocks, 256, 0, s, p, shared, own_parts)
+            : launch_pdl(attention_join_kernel<128, false>, blocks, 256, 0, s, p, shared, own_parts);
   else
-    ce = bf ? launch_pdl(attention_join_kernel<64, true>, blocks, 256, 0, s, p, parts)
-            : launch_pdl(attention_join_kernel<64, false>, blocks, 256, 0, s, p, parts);
+    ce = bf ? launch_pdl(attention_join_kernel<64, true>, blocks, 256, 0, s, p, shared, own_parts)
+            : launch_pdl(attention_join_kernel<64, false>, blocks, 256, 0, s, p, shared, own_parts);
   if (ce != cudaSuccess) return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
@@ -223,9 +289,9 @@ extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_d
     st = launch_attention_tiles(p, a.shared, bf, a.shared_tiles, s);
     if (st != VQB_OK) return st;
   }
-  st = a.decode ? launch_attention_decode(p, a.own, bf, s) : launch_attention_tiles(p, a.own, bf, a.own_tiles, s);
+  st = a.decode ? launch_attention_decode(p, a.own, a.shared, bf, s) : launch_attention_tiles(p, a.own, bf, a.own_tiles, s);
   if (st != VQB_OK) return st;
-  if (a.join) st = launch_join(p, a.parts, bf, s);
+  if (a.join) st = launch_join(p, a.shared, a.own.splits, bf, s);
   timer_after(s);
   return st;
 }

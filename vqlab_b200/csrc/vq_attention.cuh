@@ -33,15 +33,24 @@ struct AttnParams {
 struct AttnPass {
   int joint;     // rows of all requests together, over the shared prefix alone
   int prefix;    // (not joint) the request's keys begin with the shared prefix
-  int splits;
+  int splits;    // 0: no such pass
+  int rest;      // (joint) splits of the last pair of tiles, when only one of the two has rows; 0: as the others
   int part0;     // first partial result of the pass, one a split; -1: the pass writes out itself
   int cluster;   // decode kernel: blocks of a cluster, which share a split's keys
-  int joins;     // decode kernel: partial results 0 .. joins - 1 to join with its own
   int first;     // the call's first pass: its first block clears the status block
 };
 
-vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, unsigned tiles, cudaStream_t s);
-vqb_status launch_attention_decode(const AttnParams& p, const AttnPass& pass, bool bf16, cudaStream_t s);
+// Rows of a key/value head that one block of the tile kernel takes.
+constexpr int kPairRows = 256;
+
+// Partial results of the pass over the prefix that a row has: `row` counts the
+// rows of its key/value head (token * group + head of the group).
+__device__ __forceinline__ int shared_parts(const AttnPass& shared, int rows, int64_t row) {
+  return shared.rest && row >= static_cast<int64_t>(rows / kPairRows) * kPairRows ? shared.rest : shared.splits;
+}
+
+vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, int64_t tiles, cudaStream_t s);
+vqb_status launch_attention_decode(const AttnParams& p, const AttnPass& pass, const AttnPass& shared, bool bf16, cudaStream_t s);
 
 constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum follows the scores only when they pass it by this many

@@ -33,8 +33,17 @@ template <int D>
 constexpr int kHalfBytes = kUnit * D * 2;  // K or V of a stage
 template <int D>
 constexpr size_t kRingBytes = size_t(kStages<D>) * 2 * kHalfBytes<D>;  // of a warp; at the end fp32 [16][D]
+
+// A block's shared memory: the rings first (1024-byte aligned, as the copies'
+// swizzle needs: the block has no other shared memory), then the small things.
 template <int D>
-constexpr size_t decode_smem() { return 1024 + kWarps * kRingBytes<D>; }
+struct DecodeSmem {
+  unsigned char rings[kWarps * kRingBytes<D>];
+  uint64_t full[kWarps][kStages<D>];
+  float2 ml[16];  // the block's own
+  float m[kWarps][16], l[kWarps][16];
+  int abort;
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -104,15 +113,16 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kWarps * 32, kResident<D>)
-attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
+attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap) {
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t s_full[kWarps][kStages<D>];
-  __shared__ float s_m[kWarps][16], s_l[kWarps][16];
-  __shared__ float2 s_ml[16];  // the block's own
-  __shared__ int s_abort;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  DecodeSmem<D>& sm = *reinterpret_cast<DecodeSmem<D>*>(smem);
+  auto& s_full = sm.full;
+  auto& s_m = sm.m;
+  auto& s_l = sm.l;
+  auto& s_ml = sm.ml;
+  int& s_abort = sm.abort;
   constexpr int NS = kStages<D>;
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const vqb_attention_desc& d = p.d;
   if (threadIdx.x == 0) {
@@ -134,8 +144,11 @@ attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUt
   const int cluster = blockIdx.x / ranks;
   const RequestRows rq = request_rows(p, r);
   const int nrows = min(rq.nq * p.group, 16);
+  // Whoever waits for this kernel also waits for the pass before it, through the
+  // first block; the others may leave before that pass has ended.
+  const bool waits = !pass.first && (blockIdx.x | blockIdx.y | blockIdx.z) == 0;
   if (nrows == 0) {  // the same for the whole cluster
-    if (!pass.first) pdl_wait();  // whoever waits for this kernel also waits for the pass before it
+    if (waits) pdl_wait();
     return;
   }
   const int seg0 = pass.prefix ? d.prefix_len : 0;
@@ -350,8 +363,9 @@ attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUt
       *reinterpret_cast<float4*>(p.part_o + at * D + e) = j.o;
       if (e == 0) p.part_ml[at] = make_float2(j.m, j.l);
     } else {
+      const int joins = pass.first ? 0 : shared_parts(shared, d.n_tokens * p.group, tok * p.group + row % p.group);
 #pragma unroll 4
-      for (int i2 = 0; i2 < pass.joins; ++i2) {
+      for (int i2 = 0; i2 < joins; ++i2) {
         const int64_t at = i2 * all_rows + grow;
         const float2 ml = __ldcg(p.part_ml + at);
         j.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + e)));
@@ -363,12 +377,12 @@ attention_decode_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUt
     }
   }
   if (ranks > 1) cluster_sync();  // no block leaves while another reads its memory
-  if (!pass.first && partial) pdl_wait();
+  if (waits) pdl_wait();
 }
 
 template <int D, bool BF16>
-vqb_status launch(const AttnParams& p, const AttnPass& pass, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
-  constexpr size_t smem = decode_smem<D>();
+vqb_status launch(const AttnParams& p, const AttnPass& pass, const AttnPass& shared, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  constexpr size_t smem = sizeof(DecodeSmem<D>);
   if (cudaFuncSetAttribute(attention_decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
@@ -386,22 +400,22 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, const CUtensorMap& 
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, attention_decode_kernel<D, BF16>, p, pass, km, vm) != cudaSuccess) return VQB_CUDA_ERROR;
+  if (cudaLaunchKernelEx(&cfg, attention_decode_kernel<D, BF16>, p, pass, shared, km, vm) != cudaSuccess) return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
 }
 
 }  // namespace
 
-vqb_status launch_attention_decode(const AttnParams& p, const AttnPass& pass, bool bf16, cudaStream_t s) {
+vqb_status launch_attention_decode(const AttnParams& p, const AttnPass& pass, const AttnPass& shared, bool bf16, cudaStream_t s) {
   CUtensorMap km, vm;
   const vqb_attention_desc& d = p.d;
   vqb_status st = encode_pool(&km, d, bf16, p.kc, d.kc_page_stride, d.kc_head_stride, d.kc_token_stride, kUnit);
   if (st != VQB_OK) return st;
   st = encode_pool(&vm, d, bf16, p.vc, d.vc_page_stride, d.vc_head_stride, d.vc_token_stride, kUnit);
   if (st != VQB_OK) return st;
-  if (d.head_dim == 128) return bf16 ? launch<128, true>(p, pass, km, vm, s) : launch<128, false>(p, pass, km, vm, s);
-  return bf16 ? launch<64, true>(p, pass, km, vm, s) : launch<64, false>(p, pass, km, vm, s);
+  if (d.head_dim == 128) return bf16 ? launch<128, true>(p, pass, shared, km, vm, s) : launch<128, false>(p, pass, shared, km, vm, s);
+  return bf16 ? launch<64, true>(p, pass, shared, km, vm, s) : launch<64, false>(p, pass, shared, km, vm, s);
 }
 
 }  // namespace vqb

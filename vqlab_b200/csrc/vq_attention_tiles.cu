@@ -35,7 +35,7 @@
 namespace vqb {
 namespace {
 
-constexpr int kTileRows = 128;
+constexpr int kTileRows = kPairRows / 2;
 constexpr int kTileKeys = 128;
 constexpr int kThreads = 352;
 constexpr int kWarpQk = 8, kWarpPv = 9, kWarpTma = 10;
@@ -218,7 +218,7 @@ struct TileWork {
 // blocks count pairs of tiles over the requests, the last first (a causal
 // prompt's last tiles have the most keys).  false: nothing there.
 __device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& pass, int block, int lane, TileWork* w) {
-  constexpr int kRows = 2 * kTileRows;
+  constexpr int kRows = kPairRows;
   const vqb_attention_desc& d = p.d;
   if (pass.joint) {
     w->request = -1;
@@ -308,11 +308,17 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   clear_status(p, pass);
   pdl_trigger();
   TileWork w;
-  if (!find_work(p, pass, blockIdx.x / d.kv_heads, lane, &w)) return;  // the same for every thread
-  const int kvh = blockIdx.x % d.kv_heads, split = blockIdx.y;
+  // block (tile pair, split): the splits of a pair are neighbours; a last pair of one tile may have fewer
+  const int item = blockIdx.x / d.kv_heads, kvh = blockIdx.x % d.kv_heads;
+  const int pairs_full = pass.rest ? (d.n_tokens * p.group) / kPairRows : 0x7fffffff;
+  const bool in_rest = item / pass.splits >= pairs_full;
+  const int splits = in_rest ? pass.rest : pass.splits;
+  const int tile_pair = in_rest ? pairs_full : item / pass.splits;
+  const int split = in_rest ? item - pairs_full * pass.splits : item - tile_pair * pass.splits;
+  if (!find_work(p, pass, tile_pair, lane, &w)) return;  // the same for every thread
   const int tiles0 = (w.seg0 + kTileKeys - 1) / kTileKeys, all = tiles0 + (w.seg1 + kTileKeys - 1) / kTileKeys;
-  const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / pass.splits);
-  const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / pass.splits) - t0;
+  const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
+  const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - t0;
   const int active = w.rows - w.row0 > kTileRows ? 2 : 1;
 
   uint32_t tmem = 0;
@@ -323,14 +329,22 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (warp < kWarpQk) {
       // Q into shared memory (128-byte swizzle), rows past the last as zeros; K's first tiles are on their way meanwhile
-#pragma unroll 4
-      for (int i = threadIdx.x; i < active * kTileRows * (D / 8); i += kWarpQk * 32) {
-        const int row = i / (D / 8), c = i % (D / 8), g = w.row0 + row, gq = min(g, w.rows - 1), tok = gq / p.group;
-        const uint16_t* src = p.q + (w.rq.q0 + tok) * d.q_token_stride + (kvh * p.group + (gq - tok * p.group)) * d.q_head_stride + c * 8;
-        const int tr = row & (kTileRows - 1);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                     :: "r"(smem_u32(q_s + (row / kTileRows) * kQTile + (c >> 3) * kHalf + tr * 128 + (((c & 7) ^ (tr & 7)) << 4))),
-                        "l"(src), "r"(g < w.rows ? 16 : 0) : "memory");
+      // (a warp loads its 32 rows, a lane knowing where one of them is)
+      const int g = w.row0 + warp * 32 + lane, gq = min(g, w.rows - 1), tok = gq / p.group;
+      const unsigned long long mine = reinterpret_cast<unsigned long long>(
+          p.q + (w.rq.q0 + tok) * d.q_token_stride + (kvh * p.group + (gq - tok * p.group)) * d.q_head_stride);
+      constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks;
+      const int c = lane % kChunks;
+      const int nlive = min(max(w.rows - (w.row0 + warp * 32), 0), 32);
+      const uint32_t to = smem_u32(q_s + (warp >> 2) * kQTile + (c >> 3) * kHalf + (warp & 3) * 32 * 128);
+      if (warp < 4 * active) {
+#pragma unroll
+        for (int r = 0; r < 32; r += kAtOnce) {
+          const int row = r + lane / kChunks;
+          const unsigned long long src = __shfl_sync(0xffffffffu, mine, row) + c * 16;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       :: "r"(to + row * 128 + (((c & 7) ^ (row & 7)) << 4)), "l"(src), "r"(row < nlive ? 16 : 0) : "memory");
+        }
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -618,7 +632,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
             __syncwarp();
           }
           const int nlive = min(max(w.rows - (g - lane), 0), 32);  // rows of the warp that exist
-#pragma unroll 4
+#pragma unroll
           for (int r = 0; r < 32; r += 32 / kRowChunks) {
             const int rr = r + lane / kRowChunks, c = lane % kRowChunks;
             const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), rr);
@@ -642,7 +656,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
 }
 
 template <int D, bool BF16>
-vqb_status launch(const AttnParams& p, const AttnPass& pass, unsigned tiles, const CUtensorMap& km, const CUtensorMap& vm,
+vqb_status launch(const AttnParams& p, const AttnPass& pass, int64_t tiles, const CUtensorMap& km, const CUtensorMap& vm,
                   cudaStream_t s) {
   constexpr size_t smem = tiles_smem<D>();
   static_assert(smem <= 232448, "over the opt-in shared memory of an SM");
@@ -650,7 +664,10 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, unsigned tiles, con
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
   // the rows with the most keys first, over all heads
-  const dim3 grid(tiles * p.d.kv_heads, pass.splits);
+  const int64_t items = pass.rest ? static_cast<int64_t>(tiles - 1) * pass.splits + pass.rest
+                                  : static_cast<int64_t>(tiles) * pass.splits;
+  if (items * p.d.kv_heads > 0x7fffffff) return VQB_UNSUPPORTED_GEOMETRY;
+  const dim3 grid(static_cast<unsigned>(items * p.d.kv_heads));
   if (launch_pdl(attention_tiles_kernel<D, BF16>, grid, kThreads, smem, s, p, pass, km, vm) != cudaSuccess)
     return VQB_CUDA_ERROR;
   note_launch();
@@ -660,7 +677,7 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, unsigned tiles, con
 }  // namespace
 
 // tiles: an upper bound of the pairs of row tiles of the pass.
-vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, unsigned tiles, cudaStream_t s) {
+vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, int64_t tiles, cudaStream_t s) {
   CUtensorMap km, vm;
   const vqb_attention_desc& d = p.d;
   const int box = d.page_size < kTileKeys ? d.page_size : kTileKeys;
