@@ -105,6 +105,27 @@ class Case:
                 assert bool(((ml - L).abs()[~inf] <= (ds + 2.0 ** -16 + 2.0 ** -22 * L.abs())[~inf]).all())
         return got
 
+    def reference(self):
+        """(result, bound) [N, heads, D] in 64 bits of a causal call at the default scale."""
+        u, G, cu = HALF_UNIT[self.dtype], self.H // self.KH, self.cu.tolist()
+        out = torch.zeros(self.q.shape, dtype=torch.double, device="cuda")
+        lim = torch.zeros_like(out)
+        for r, length in enumerate(self.lens):
+            n = cu[r + 1] - cu[r]
+            for h in range(self.KH):
+                own = self.table[r, :-(-length // self.page)]
+                k = torch.cat([self.rows(self.k, self.prefix_pages, self.prefix, h), self.rows(self.k, own, length, h)])
+                v = torch.cat([self.rows(self.v, self.prefix_pages, self.prefix, h), self.rows(self.v, own, length, h)])
+                x = self.q[cu[r]:cu[r + 1], h * G:(h + 1) * G].double().reshape(-1, self.D)
+                s = x @ k.T * self.D ** -0.5
+                ds = ((x.abs() @ k.abs().T) * self.D ** 0.5 * 2.0 ** -23 + s.abs() * 2.0 ** -22).amax(-1, keepdim=True)
+                last = self.prefix + length - n + torch.arange(n, device="cuda").repeat_interleave(G)
+                w = torch.softmax(s.masked_fill(torch.arange(k.shape[0], device="cuda")[None] > last[:, None], -torch.inf), -1)
+                o, A = w @ v, w @ v.abs()
+                out[cu[r]:cu[r + 1], h * G:(h + 1) * G] = o.view(n, G, self.D)
+                lim[cu[r]:cu[r + 1], h * G:(h + 1) * G] = (u * o.abs() + (u + 2 * ds + 2.0 ** -16) * A + 2.0 ** -25).view(n, G, self.D)
+        return out, lim
+
 
 BF, FP = torch.bfloat16, torch.float16
 
@@ -231,6 +252,74 @@ def test_loose_bounds_and_other_streams():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, c.run(max_kv_len=room)) and not torch.equal(out, first)
+
+
+@pytest.mark.parametrize("q_lens,kv,prefix", [([1] * 40, [60] * 40, 3000), ([300, 20], [300, 40], 200), ([1] * 3, [9000] * 3, 0)])
+def test_captured_graphs(q_lens, kv, prefix):
+    c = Case(q_lens, kv, prefix, 10, 2, 128, 64, BF, seed=13)
+    want = c.run()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = c.run()
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("q_len", [1, 3, 40])
+def test_nan_and_infinity_reach_the_rows_that_see_them(q_len):
+    """NaN or infinity in a key or a value makes the rows that see it what the formula says and leaves the others."""
+    for D, page, seed in ((128, 16, 14), (64, 64, 15)):
+        c = Case([q_len] * 3, [200, 130, 90], 60, 4, 2, D, page, BF, seed=seed)
+        want, lim = c.reference()
+        k0, v0 = c.k.clone(), c.v.clone()
+        for r, j in ((0, 3), (0, 127), (0, 163), (0, 199), (1, 95), (1, 129), (2, 70), (2, 89)):
+            p, o = int(c.table[r, j // page]), j % page
+            first = c.lens[r] - q_len  # place of the request's first query
+            sees = torch.zeros(want.shape[:2], dtype=torch.bool, device="cuda")
+            sees[r * q_len + max(j - first, 0):(r + 1) * q_len, 2:] = True  # key/value head 1
+            for bad in (float("nan"), float("inf"), -float("inf")):
+                c.k.copy_(k0)
+                c.v.copy_(v0)
+                c.v[p, 1, o, 5] = bad
+                got = c.run().double()
+                ok = (got - want).abs() <= lim
+                assert bool(ok[~sees].all()), ("v", r, j, bad)
+                assert bool(ok[..., :5][sees].all()) and bool(ok[..., 6:][sees].all()), ("v", r, j, bad)
+                assert bool((torch.isnan(got[..., 5][sees]) if bad != bad else got[..., 5][sees] == bad).all()), ("v", r, j, bad)
+                c.v.copy_(v0)
+                c.k[p, 1, o, 5] = bad
+                got = c.run().double()
+                assert bool(((got - want).abs() <= lim)[~sees].all()), ("k", r, j, bad)
+                x = got[sees]
+                if bad != bad:
+                    assert bool(torch.isnan(x).all()), ("k", r, j)
+                else:  # q * inf: inf, and the row is NaN, or -inf, and the key's weight is 0
+                    up = (c.q[..., 5].double() * bad)[sees] > 0
+                    assert bool(torch.isnan(x[up]).all()) and bool(torch.isfinite(x[~up]).all()), ("k", r, j, bad)
+        c.k.copy_(k0)
+        c.v.fill_(float("nan"))
+        assert bool(torch.isnan(c.run()).all())
+
+
+@pytest.mark.parametrize("q_lens,kv,prefix", [([1, 1], [100, 60], 40), ([70, 3], [100, 60], 200)])
+def test_offsets_past_32_bits(q_lens, kv, prefix):
+    """A pool of over 2^32 bytes and 2^31 elements, the pages in use at its end."""
+    c = Case(q_lens, kv, prefix, 4, 2, 128, 64, FP, seed=15)
+    want = c.run()
+    n, far = c.k.shape[0], 140000
+    big = [torch.empty((far, 2, 64, 128), dtype=FP, device="cuda") for _ in range(2)]
+    assert big[0].numel() > 2 ** 31
+    for b, x in zip(big, (c.k, c.v)):
+        b[far - n:] = x
+    c.k, c.v = big
+    c.table = torch.where(c.table >= 0, c.table + (far - n), -1).to(torch.int32)
+    c.prefix_pages = (c.prefix_pages + (far - n)).to(torch.int32)
+    assert torch.equal(c.run(), want)
 
 
 def test_pages_outside_the_pool_read_as_zeros():

@@ -117,6 +117,22 @@ def test_unaligned_and_strided(shift):
     assert torch.equal(vc.transpose(1, 2).reshape(-1, KH, D)[20:20 + N], v)
 
 
+def test_slots_past_32_bits():
+    """A pool of over 2^31 elements, the slots at its end."""
+    q, k, v, _, _ = tensors(5, 4, 2, 128, torch.float16, 64, 1, 3)
+    pages = 140000
+    kc, vc = (torch.empty((pages, 2, 64, 128), dtype=torch.float16, device="cuda") for _ in range(2))
+    assert kc.numel() > 2 ** 31
+    freq, _ = rotary_frequencies(128)
+    pos = torch.arange(5, dtype=torch.int32, device="cuda")
+    slots = (pages * 64 - 1 - 13 * torch.arange(5, device="cuda")).to(torch.int32)
+    rotary_append(q, k, v, pos, freq, kc, vc, slots)
+    want, size = reference(k, pos, freq, False, 1.0)
+    page, off = (slots // 64).long(), (slots % 64).long()
+    close(kc[page, :, off], want, size, torch.float16)
+    assert torch.equal(vc[page, :, off], v)
+
+
 def test_rotation_keeps_relative_scores():
     """q.k after rotation depends on the positions' difference alone, also at far positions."""
     freq, _ = rotary_frequencies(128, 1e6)

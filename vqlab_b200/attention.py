@@ -223,4 +223,4 @@ class VQAttention(torch.nn.Module):
         o = prefix_attention(q, kc, vc, step.block_table, step.kv_lens, step.cu_q, max_q_len=max_q_len,
                              max_kv_len=max_kv_len, prefix_pages=cache.prefix_pages, prefix_len=cache.prefix_len,
                              scale=self.scale)
-        return self.o_proj(o.view(N, -1))
+        return self.o_proj(o.view(N, self.heads * self.head_dim))

@@ -207,6 +207,107 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, AttnP
   if (p.lse && lane == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+// ---- rows that a masked value has spoiled (0 times a value that is not finite)
+
+template <bool BF16>
+__device__ __forceinline__ float widen16(uint16_t h) {
+  if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(h) << 16);
+  else return __half2float(__ushort_as_half(h));
+}
+
+// A row that is not finite, of a request whose later keys it does not see: worked out
+// again, by a warp, over the keys that it does see -- if one of the values that it
+// does not see is indeed not finite.  A row that is not finite by what it sees stays so.
+template <int D, bool BF16>
+__device__ void exact_row(const AttnParams& p, int request, const RequestRows& rq, int64_t token, int head) {
+  const vqb_attention_desc& d = p.d;
+  const int lane = threadIdx.x & 31, kvh = head / p.group;
+  const int seen = visible(p, rq, static_cast<int>(token) - rq.q0);
+  auto page_of = [&](bool own, int j) {
+    const int page = own ? __ldg(p.table + static_cast<int64_t>(request) * d.table_width + (j >> p.page_shift))
+                         : __ldg(p.prefix_pages + (j >> p.page_shift));
+    return static_cast<unsigned>(page) < static_cast<unsigned>(d.num_pages) ? page : -1;
+  };
+  auto value = [&](int page, int j) {
+    return p.vc + page * d.vc_page_stride + kvh * d.vc_head_stride + (j & (d.page_size - 1)) * d.vc_token_stride;
+  };
+  bool fault = false;
+  for (int j0 = seen; j0 < rq.len && !fault; j0 += 32) {
+    const int j = j0 + lane;
+    bool bad = false;
+    const int page = j < rq.len ? page_of(true, j) : -1;
+    if (page >= 0) {
+      const uint16_t* v = value(page, j);
+      for (int e = 0; e < D; ++e) bad = bad || !(fabsf(widen16<BF16>(v[e])) < INFINITY);
+    }
+    fault = __any_sync(0xffffffffu, bad);
+  }
+  if (!fault) return;
+  const uint16_t* q = p.q + token * d.q_token_stride + head * d.q_head_stride;
+  float acc[D / 32];
+  float m = -INFINITY, l = 0.0f;
+  for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
+  bool nan = false;  // NaN it stays, whatever follows
+  for (int part = 0; part < 2; ++part) {
+    const int end = part ? seen : d.prefix_len;
+    for (int j0 = 0; j0 < end && !nan; j0 += 32) {
+      const int j = j0 + lane;
+      const int page = j < end ? page_of(part != 0, j) : -1;
+      float s = j < end ? 0.0f : -INFINITY;
+      if (page >= 0) {
+        const uint16_t* k = p.kc + page * d.kc_page_stride + kvh * d.kc_head_stride + (j & (d.page_size - 1)) * d.kc_token_stride;
+        for (int e = 0; e < D; ++e) s = fmaf(widen16<BF16>(q[e]), widen16<BF16>(k[e]), s);
+      }
+      s *= p.scale_log2;
+      float top = s;
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
+      const float keep = exp2f(m - base), w = j < end ? exp2f(s - base) : 0.0f;
+      m = mn;
+      float sum = w;
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l = l * keep + sum;
+      bool all_nan = true;
+      for (int e = 0; e < D / 32; ++e) acc[e] *= keep;
+      for (int i = 0; i < 32; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        const int pg = __shfl_sync(0xffffffffu, page, i);
+        if (pg < 0) continue;
+        const uint16_t* v = value(pg, j0 + i);
+        for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wi, widen16<BF16>(v[lane + 32 * e]), acc[e]);
+      }
+      for (int e = 0; e < D / 32; ++e) all_nan = all_nan && acc[e] != acc[e];
+      nan = l != l || __all_sync(0xffffffffu, all_nan);
+    }
+  }
+  uint16_t* out = p.out + token * d.out_token_stride + head * d.out_head_stride;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  for (int e = 0; e < D / 32; ++e) out[lane + 32 * e] = narrow16<BF16>(acc[e] * inv);
+  if (p.lse && lane == 0) p.lse[token * d.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// After the passes of a call that masks keys: nothing, unless a pass noted a row
+// that is not finite.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attention_exact_kernel(AttnParams p) {
+  pdl_wait();
+  pdl_trigger();
+  if (__ldcg(p.status + 1) == 0) return;
+  const vqb_attention_desc& d = p.d;
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = static_cast<int64_t>(min(__ldg(p.cu_q + d.n_requests), d.n_tokens)) * d.heads;
+  for (int64_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8) {
+    const int64_t n = row / d.heads;
+    const int h = static_cast<int>(row - n * d.heads);
+    const uint16_t* out = p.out + n * d.out_token_stride + h * d.out_head_stride;
+    bool bad = false;
+    for (int e = lane; e < D; e += 32) bad = bad || !(fabsf(widen16<BF16>(out[e])) < INFINITY);
+    if (!__any_sync(0xffffffffu, bad)) continue;
+    const int r = request_of(p.cu_q, d.n_requests, static_cast<int>(n));
+    exact_row<D, BF16>(p, r, request_rows(p, r), n, h);
+  }
+}
+
 vqb_status launch_join(const AttnParams& p, const AttnPass& shared, int own_parts, bool bf, cudaStream_t s) {
   const unsigned blocks = static_cast<unsigned>((part_rows(p.d) + 7) / 8);
   cudaError_t ce;
@@ -216,6 +317,21 @@ vqb_status launch_join(const AttnParams& p, const AttnPass& shared, int own_part
   else
     ce = bf ? launch_pdl(attention_join_kernel<64, true>, blocks, 256, 0, s, p, shared, own_parts)
             : launch_pdl(attention_join_kernel<64, false>, blocks, 256, 0, s, p, shared, own_parts);
+  if (ce != cudaSuccess) return VQB_CUDA_ERROR;
+  note_launch();
+  return VQB_OK;
+}
+
+vqb_status launch_exact(const AttnParams& p, bool bf, cudaStream_t s) {
+  const size_t rows = (part_rows(p.d) + 7) / 8;
+  const unsigned blocks = static_cast<unsigned>(rows < 296 ? rows : 296);
+  cudaError_t ce;
+  if (p.d.head_dim == 128)
+    ce = bf ? launch_pdl(attention_exact_kernel<128, true>, blocks, 256, 0, s, p)
+            : launch_pdl(attention_exact_kernel<128, false>, blocks, 256, 0, s, p);
+  else
+    ce = bf ? launch_pdl(attention_exact_kernel<64, true>, blocks, 256, 0, s, p)
+            : launch_pdl(attention_exact_kernel<64, false>, blocks, 256, 0, s, p);
   if (ce != cudaSuccess) return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
@@ -292,6 +408,7 @@ extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_d
   st = a.decode ? launch_attention_decode(p, a.own, a.shared, bf, s) : launch_attention_tiles(p, a.own, bf, a.own_tiles, s);
   if (st != VQB_OK) return st;
   if (a.join) st = launch_join(p, a.shared, a.own.splits, bf, s);
+  if (st == VQB_OK && d.causal && d.max_q_len > 1) st = launch_exact(p, bf, s);
   timer_after(s);
   return st;
 }

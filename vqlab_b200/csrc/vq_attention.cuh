@@ -23,7 +23,7 @@ struct AttnParams {
   float* lse;
   float* part_o;
   float2* part_ml;
-  int* status;      // int32 [1] of the workspace
+  int* status;      // int32 [1] of the workspace; [2]: a masked value may have spoiled a row
   int group;
   int page_shift;
   float scale_log2;  // scale * log2(e): scores in powers of two
@@ -82,6 +82,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ void clear_status(const AttnParams& p, const AttnPass& pass) {
   if (pass.first && (blockIdx.x | blockIdx.y | blockIdx.z) == 0 && threadIdx.x < 4) p.status[static_cast<int>(threadIdx.x) - 1] = 0;
 }
+
+// The MMAs multiply a masked value by a weight of 0, which is NaN where the value is
+// not finite.  A pass that masks keys says here that a row of it came out not
+// finite; a kernel after the passes then works such rows out again (vq_attention.cu).
+__device__ __forceinline__ void note_not_finite(const AttnParams& p) { p.status[1] = 1; }
 
 // The queries of request r, as far as the call's bounds go.
 struct RequestRows {

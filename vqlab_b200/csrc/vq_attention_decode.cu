@@ -358,6 +358,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
     const int64_t tok = rq.q0 + row / p.group;
     const int head = kvh * p.group + row % p.group;
     const int64_t grow = tok * d.heads + head;
+    if (visible(p, rq, row / p.group) < seg1 && (j.o.x + j.o.y + j.o.z + j.o.w) * 0.0f != 0.0f) note_not_finite(p);
     if (partial) {
       const int64_t at = (pass.part0 + cluster) * all_rows + grow;
       *reinterpret_cast<float4*>(p.part_o + at * D + e) = j.o;

@@ -602,6 +602,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         unsigned char* stage = q_s + t * kQTile + (warp & 3) * 32 * kRowBytes;
         unsigned char* mine = partial ? reinterpret_cast<unsigned char*>(p.part_o + at * D)
                                       : reinterpret_cast<unsigned char*>(p.out + token * d.out_token_stride + head * d.out_head_stride);
+        float zero = 0.0f;  // NaN once an element is not finite
         for (int pass2 = 0; pass2 < (partial ? 2 : 1); ++pass2) {
           const int cols = partial ? D / 2 : D;
 #pragma unroll 1
@@ -614,6 +615,8 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = 0u;
             }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) zero = fmaf(__uint_as_float(o[e]), 0.0f, zero);
             if (partial) {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
@@ -642,6 +645,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
           }
           __syncwarp();
         }
+        if (live && vis < w.seg1 && zero != 0.0f) note_not_finite(p);
         if (live) {
           if (partial) p.part_ml[at] = make_float2(m, l);
           else if (p.lse) p.lse[grow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
