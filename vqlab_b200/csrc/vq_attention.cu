@@ -102,16 +102,18 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   a.own.prefix = !joint && d.prefix_len > 0;
   if (a.decode) {
     // About two rounds of three blocks an SM, so that ragged lengths even out, each
-    // with 512 keys or more: up to 8 blocks a (request, head) in a cluster, and
-    // several clusters only where 8 would leave SMs idle.
+    // with 512 keys or more (128 where that leaves SMs idle): up to 8 blocks a
+    // (request, head) in a cluster, and several clusters only where 8 would leave
+    // SMs idle.
     int64_t s = ceil_div(6 * sms, requests_heads);
-    if (s > ceil_div(keys, 512)) s = ceil_div(keys, 512);
+    const int64_t most_s = ceil_div(keys, requests_heads * ceil_div(keys, 512) < sms ? 128 : 512);
+    if (s > most_s) s = most_s;
     a.own.cluster = 1;
     while (a.own.cluster < 8 && a.own.cluster * 2 <= s) a.own.cluster *= 2;
     a.own.splits = 1;
-    if (requests_heads * 8 < sms && s > 8) {
-      s = ceil_div(2 * sms, requests_heads * 8) < s / 8 ? ceil_div(2 * sms, requests_heads * 8) : s / 8;
-      a.own.splits = static_cast<int>(s < 16 ? s : 16);
+    if (requests_heads * 8 < sms && keys > 8 * 512) {  // a join kernel pays from about 500 keys a block on
+      const int64_t fill = ceil_div(2 * sms, requests_heads * 8), most_k = keys / (8 * 256);
+      a.own.splits = static_cast<int>(fill < most_k ? fill : most_k);
     }
   } else {
     a.own_tiles = rows / kPairRows + d.n_requests;

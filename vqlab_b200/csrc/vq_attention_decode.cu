@@ -135,9 +135,17 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
   // With a pass over the prefix before this kernel, that pass's blocks have all
   // waited for what came before them by the time this one may start, and only its
   // results have to be waited for, below.
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+  }
   if (pass.first) pdl_wait();
   pdl_trigger();
   clear_status(p, pass);
+  // the request's table row is on its way while its lengths are read
+  if (static_cast<int>(threadIdx.x) * 32 < d.table_width)
+    asm volatile("prefetch.global.L1 [%0];"
+                 :: "l"(p.table + static_cast<int64_t>(blockIdx.z) * d.table_width + threadIdx.x * 32) : "memory");
 
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
   const int kvh = blockIdx.y, r = blockIdx.z;
