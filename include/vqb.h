@@ -7,7 +7,8 @@
  *
  * Every pointer is a DEVICE pointer owned by the caller.  The compute entry
  * points (vqb_unpack, vqb_codebook_halves, vqb_switch_forward[_static],
- * vqb_dense_forward, the MoE elementwise calls, vqb_moe_block_forward and
+ * vqb_dense_forward, the MoE elementwise calls, vqb_moe_block_forward,
+ * vqb_paged_tables, vqb_rotary_append, vqb_prefix_attention and
  * vqb_ep_dispatch / combine / reduce) are asynchronous on the given stream and
  * allocate nothing; calls
  * that need scratch memory take a caller-supplied workspace whose size the
@@ -476,7 +477,8 @@ vqb_status vqb_rotary_append(const vqb_rotary_desc* desc, vqb_dtype dtype, const
  * lse (optional, fp32 [n_tokens, heads]): log of the sum of exp of the scaled
  * scores (-inf for such a row).  Rows past cu_q[n_requests] are not written.
  * Cache places past a request's length are never used, whatever they hold; a
- * page outside the pool reads as zeros.
+ * page outside the pool reads as zeros.  A key or value that is not finite
+ * makes the rows that see it what the formula says, and no other.
  *
  * max_q_len / max_kv_len bound the requests' queries and own tokens (the
  * lengths themselves are on the device): what lies past them is left out.
