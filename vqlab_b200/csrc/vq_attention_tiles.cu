@@ -28,8 +28,6 @@
 //
 // Every wait is bounded (2 s): on expiry the block records VQB_TIMEOUT, waits for
 // its copies and MMAs in flight, frees its tensor memory and returns.
-#include <type_traits>
-
 #include "vq_attention.cuh"
 
 namespace vqb {
@@ -146,35 +144,37 @@ __device__ __forceinline__ float max128(const float* s) {
 
 // 2^x of two numbers on the FMA pipe: x = n + f with n the nearest integer (adding
 // 1.5 * 2^23 leaves n in the sum's low bits), 2^f for f in [-1/2, 1/2] by a
-// polynomial of degree 4 (Remez, relative error 2^-18.5, below the weights' 16
-// bits), n added to the exponent.  x below -126 gives about 2^-126.
+// polynomial of degree 4 (least relative error with the constant 1: 2^-18.4, below
+// the weights' 16 bits), n added to the exponent.  x is held to -127, for which the
+// sum of the bits of 1 and of -127 in the exponent is 0: masked scores (-inf) get
+// weight 0.
 __device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
   float2 x = unpair(x2);
-  x2 = pair(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+  x2 = pair(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
   const uint64_t magic = pair(12582912.0f, 12582912.0f), unmagic = pair(-12582912.0f, -12582912.0f);
   const uint64_t t = add2(x2, magic);
   const uint64_t f = fma2(add2(t, unmagic), pair(-1.0f, -1.0f), x2);
-  uint64_t r = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
-  r = fma2(r, f, pair(0.240247443318367f, 0.240247443318367f));
-  r = fma2(r, f, pair(0.6931217908859253f, 0.6931217908859253f));
-  r = fma2(r, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  uint64_t r = fma2(f, pair(0.009582818485796452f, 0.009582818485796452f), pair(0.05590637028217316f, 0.05590637028217316f));
+  r = fma2(r, f, pair(0.24024099111557007f, 0.24024099111557007f));
+  r = fma2(r, f, pair(0.6931241750717163f, 0.6931241750717163f));
+  r = fma2(r, f, pair(1.0f, 1.0f));
   const float2 y = unpair(r), k = unpair(t);
   return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(k.x) << 23)),
                      __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(k.y) << 23)));
 }
 
 // Weights 2^(score * scale - base) of 32 scores as 16-bit numbers; returns their
-// sum.  EVERY > 0: every EVERY-th pair on the FMA pipe, which is otherwise little
+// sum.  Every kPolyEvery-th pair goes to the FMA pipe, which is otherwise little
 // used, since the special function unit's 16 exponentials a cycle bound a tile as
 // much as its MMAs do.
-template <bool BF16, int EVERY>
+template <bool BF16>
 __device__ __forceinline__ float weights32(uint32_t (&pk)[16], const float* s, uint64_t scale2, uint64_t base2) {
   uint64_t sum0 = pair(0.f, 0.f), sum1 = sum0;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const uint64_t x2 = fma2(pair(s[2 * e], s[2 * e + 1]), scale2, base2);
     float2 w;
-    if (EVERY > 0 && e % (EVERY > 0 ? EVERY : 1) == EVERY - 1) {
+    if (e % kPolyEvery == kPolyEvery - 1) {
       w = exp2_poly(x2);
     } else {
       const float2 x = unpair(x2);
@@ -513,8 +513,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_read[t]);
-        const bool mask = __any_sync(0xffffffffu, lim < kTileKeys);
-        if (mask) {
+        if (__any_sync(0xffffffffu, lim < kTileKeys)) {
 #pragma unroll
           for (int c = 0; c < 128; ++c)
             if (c >= lim) s[c] = -INFINITY;
@@ -543,29 +542,20 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         }
         const float base = m == -INFINITY ? 0.0f : m;
         const uint64_t base2 = pair(-base, -base);
+        uint32_t pk0[16], pk1[16];
+        l += weights32<BF16>(pk0, s, scale2, base2);
+        l += weights32<BF16>(pk1, s + 32, scale2, base2);
         // the weights of the key tile before have met their values once its MMAs are done
-        auto weights = [&](auto every) {
-          constexpr int kEvery = decltype(every)::value;
-          uint32_t pk0[16], pk1[16];
-          l += weights32<BF16, kEvery>(pk0, s, scale2, base2);
-          l += weights32<BF16, kEvery>(pk1, s + 32, scale2, base2);
-          if (!fresh) {
-            ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag);
-            tc_fence_after();
-          }
-          if (ok) {
-            tc_st16(prow, pk0);
-            tc_st16(prow + 16, pk1);
-            l += weights32<BF16, kEvery>(pk0, s + 64, scale2, base2);
-            tc_st16(prow + 32, pk0);
-            l += weights32<BF16, kEvery>(pk1, s + 96, scale2, base2);
-            tc_st16(prow + 48, pk1);
-          }
-        };
-        // masked scores have weight 0, not 2^-126
-        if (mask) weights(std::integral_constant<int, 0>{});
-        else weights(std::integral_constant<int, kPolyEvery>{});
-        if (!ok) break;
+        if (!fresh) {
+          if (!(ok = warp_wait(&o_full[t], (i - 1) & 1, abort_flag))) break;
+          tc_fence_after();
+        }
+        tc_st16(prow, pk0);
+        tc_st16(prow + 16, pk1);
+        l += weights32<BF16>(pk0, s + 64, scale2, base2);
+        tc_st16(prow + 32, pk0);
+        l += weights32<BF16>(pk1, s + 96, scale2, base2);
+        tc_st16(prow + 48, pk1);
         // NaN or inf among the scores: NaN, also where the polynomial clamped it
         if (!(mx < INFINITY)) l = __int_as_float(0x7FC00000);
         if (t == 0 && (warp & 3) == 0 && (held & 15)) {
