@@ -26,8 +26,8 @@ struct AttnPlan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Times in microseconds, measured at D = 128: a key tile of a block with two row
-// tiles, with one, and a block's start and end.
+// Times in microseconds: a key tile of a block with two row tiles (D = 64: of one of
+// two blocks on an SM), with one, and a block's start and end.
 constexpr double kPairTile = 1.5, kOneTile = 1.2, kBlockEnds = 7.0;
 constexpr int kMaxSplits = 64;
 
@@ -89,12 +89,14 @@ bool pick_shared_splits(AttnPass* a, int64_t full, bool rest, int heads, int64_t
 
 AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   AttnPlan a{};
+  const int block_rows = tile_block_rows(d.head_dim);
+  const int slots = d.head_dim == 128 ? sms : 2 * sms;  // blocks of the tile kernel at a time
   const int group = d.heads / d.kv_heads;
   const int64_t rows = static_cast<int64_t>(d.n_tokens) * group;  // of one key/value head
   const int64_t most = static_cast<int64_t>(d.max_q_len < d.n_tokens ? d.max_q_len : d.n_tokens) * group;
   a.decode = most <= 16;
   // the prefix for all rows at once, unless a request fills tiles by itself
-  const bool joint = d.prefix_len > 0 && d.n_requests > 1 && most <= kPairRows;
+  const bool joint = d.prefix_len > 0 && d.n_requests > 1 && most <= 256;
   // a partial result written and read, at 4 TB/s
   const double row_cost = static_cast<double>(d.n_tokens) * d.heads * d.head_dim * 8.0 / 4.0e6;
   const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
@@ -116,25 +118,26 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
       a.own.splits = static_cast<int>(fill < most_k ? fill : most_k);
     }
   } else {
-    a.own_tiles = rows / kPairRows + d.n_requests;
-    const int64_t blocks = (rows / kPairRows > d.n_requests ? rows / kPairRows : d.n_requests) * d.kv_heads;
-    a.own.splits = pick_splits(blocks, ceil_div(keys, 128), sms, row_cost, joint);
+    a.own_tiles = rows / block_rows + d.n_requests;
+    const int64_t blocks = (rows / block_rows > d.n_requests ? rows / block_rows : d.n_requests) * d.kv_heads;
+    a.own.splits = pick_splits(blocks, ceil_div(keys, 128), slots, row_cost, joint);
   }
   bool together = !a.decode;  // the own pass leaves partial results too
   if (joint) {
     a.shared.joint = 1;
     a.shared.first = 1;
-    a.shared_tiles = ceil_div(rows, kPairRows);
-    const bool rest = rows % kPairRows > 0 && rows % kPairRows <= kPairRows / 2;
+    a.shared_tiles = ceil_div(rows, block_rows);
+    // the last block has one row tile with rows, of two
+    const bool rest = d.head_dim == 128 && rows % block_rows > 0 && rows % block_rows <= block_rows / 2;
     const int64_t tiles = ceil_div(d.prefix_len, 128);
     if (a.decode) {
       // an SM's time for the own keys: 100 GB/s and 2 us a block, with lengths that average 0.6 of the largest
       const double bytes = 0.6 * keys * requests_heads * d.head_dim * 4.0;
       const double other = bytes / 1.0e5 + 2.0 * requests_heads * a.own.cluster;
       const double alone = bytes / 6.4e6 > other / sms ? bytes / 6.4e6 : other / sms;
-      together = pick_shared_splits(&a.shared, a.shared_tiles - rest, rest, d.kv_heads, tiles, sms, row_cost, other, alone);
+      together = pick_shared_splits(&a.shared, a.shared_tiles - rest, rest, d.kv_heads, tiles, slots, row_cost, other * slots / sms, alone);
     } else {
-      a.shared.splits = pick_splits(a.shared_tiles * d.kv_heads, tiles, sms, row_cost, true);
+      a.shared.splits = pick_splits(a.shared_tiles * d.kv_heads, tiles, slots, row_cost, true);
     }
   }
   a.own.first = a.shared.splits == 0;
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, AttnP
   const int64_t n = row / d.heads;
   const int h = static_cast<int>(row - n * d.heads);
   if (n >= __ldg(p.cu_q + d.n_requests)) return;
-  const int ns = shared.splits ? shared_parts(shared, d.n_tokens * p.group, n * p.group + h % p.group) : 0;
+  const int ns = shared.splits ? shared_parts(shared, tile_block_rows(D), d.n_tokens * p.group, n * p.group + h % p.group) : 0;
   const int parts = ns + own_parts;  // the own pass's follow the `splits` places of the shared one's
   constexpr int kPer = D / 32;
   float m = -INFINITY, l = 0.0f, acc[kPer];

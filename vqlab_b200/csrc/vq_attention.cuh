@@ -41,12 +41,12 @@ struct AttnPass {
 };
 
 // Rows of a key/value head that one block of the tile kernel takes.
-constexpr int kPairRows = 256;
+__host__ __device__ constexpr int tile_block_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
 
 // Partial results of the pass over the prefix that a row has: `row` counts the
 // rows of its key/value head (token * group + head of the group).
-__device__ __forceinline__ int shared_parts(const AttnPass& shared, int rows, int64_t row) {
-  return shared.rest && row >= static_cast<int64_t>(rows / kPairRows) * kPairRows ? shared.rest : shared.splits;
+__device__ __forceinline__ int shared_parts(const AttnPass& shared, int block_rows, int rows, int64_t row) {
+  return shared.rest && row >= static_cast<int64_t>(rows / block_rows) * block_rows ? shared.rest : shared.splits;
 }
 
 vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, int64_t tiles, cudaStream_t s);

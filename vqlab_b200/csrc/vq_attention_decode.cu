@@ -372,7 +372,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
       *reinterpret_cast<float4*>(p.part_o + at * D + e) = j.o;
       if (e == 0) p.part_ml[at] = make_float2(j.m, j.l);
     } else {
-      const int joins = pass.first ? 0 : shared_parts(shared, d.n_tokens * p.group, tok * p.group + row % p.group);
+      const int joins = pass.first ? 0 : shared_parts(shared, tile_block_rows(D), d.n_tokens * p.group, tok * p.group + row % p.group);
 #pragma unroll 4
       for (int i2 = 0; i2 < joins; ++i2) {
         const int64_t at = i2 * all_rows + grow;

@@ -3,7 +3,7 @@
 // prefix that it shares (each prefix page is then read once for 256 rows
 // instead of once a request).
 //
-// A block takes (256 rows of one key/value head, a run of keys): two tiles of
+// A block takes (256 rows of one key/value head, 128 at D = 64, and a run of keys): two tiles of
 // 128 rows (a row = a token and a head of the group) that share every K and V
 // tile of 128 keys.  Roles:
 //   * a TMA warp fills a ring of shared-memory stages with K and V tiles, one
@@ -17,8 +17,8 @@
 //     registers, running maximum and sum, weights as 16-bit numbers to tensor
 //     memory.  O is rescaled in place, by the same thread, only when the maximum
 //     has grown by more than 2^kSlack.
-// Tensor memory's 512 columns hold two O tiles (256), two weight tiles (128) and
-// one score tile (128) that the two row tiles use in turn: it is free again as
+// Tensor memory's 512 columns (at D = 128) hold two O tiles (256), two weight tiles
+// (128) and one score tile (128) that the two row tiles use in turn: it is free again as
 // soon as the scores are in registers, so the next Q K^T runs beside this tile's
 // exponentials and no score waits for a P V.  (With a score tile each, weights
 // had to lie over scores, and each tile's chain of exponentials, P V and Q K^T was
@@ -33,19 +33,31 @@
 namespace vqb {
 namespace {
 
-constexpr int kTileRows = kPairRows / 2;
+constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-constexpr int kThreads = 352;
-constexpr int kWarpQk = 8, kWarpPv = 9, kWarpTma = 10;
-constexpr int kTmemCols = 512;
+// Row tiles of a block: two at D = 128; one at D = 64, where two blocks share an SM
+// (tensor memory then holds 256 columns of each): their starts and ends overlap, and rows
+// are dealt in 128s.
+template <int D>
+constexpr int kRowTiles = tile_block_rows(D) / kTileRows;
+// four softmax warps a row tile, then one each for Q K^T, P V and the copies
+template <int D>
+constexpr int kSoftmaxWarps = 4 * kRowTiles<D>;
+template <int D>
+constexpr int kThreads = D == 128 ? 352 : 256;
+template <int D>
+constexpr int kTmemCols = D == 128 ? 512 : 256;
+// Registers a thread at D = 64: 256 x 128 at launch; the last four warps leave 72 each,
+// which the softmax warps take: 128 x 200 + 128 x 56.
+constexpr int kRegsSoftmax = 200, kRegsOther = 56;
 constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial
 template <int D>
 constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
 template <int D>
-constexpr int kStages = D == 128 ? 5 : 8;
+constexpr int kStages = 5;
 template <int D>
 constexpr size_t tiles_smem() {
-  return 1024 + size_t(2) * kTileRows * D * 2 + size_t(kStages<D>) * kStageBytes<D> + 256;
+  return 1024 + size_t(kRowTiles<D>) * kTileRows * D * 2 + size_t(kStages<D>) * kStageBytes<D> + 256;
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -214,11 +226,11 @@ struct TileWork {
   int seg0, seg1;  // keys: of the prefix, of the request itself
 };
 
-// The block's request and rows.  joint: all tokens are one run of rows.  Else
+// The block's request and rows, kRows at a time.  joint: all tokens are one run of rows.  Else
 // blocks count pairs of tiles over the requests, the last first (a causal
 // prompt's last tiles have the most keys).  false: nothing there.
+template <int kRows>
 __device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& pass, int block, int lane, TileWork* w) {
-  constexpr int kRows = kPairRows;
   const vqb_attention_desc& d = p.d;
   if (pass.joint) {
     w->request = -1;
@@ -264,16 +276,17 @@ __device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& p
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<D>, D == 128 ? 1 : 2)
 attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char smem_raw[];
-  constexpr int NS = kStages<D>;
+  constexpr int NS = kStages<D>, NT = kRowTiles<D>;
+  constexpr int kWarpQk = kSoftmaxWarps<D>, kWarpPv = kWarpQk + 1, kWarpTma = kWarpQk + 2;
   constexpr int kHalf = kTileKeys * 128;  // 64 elements of 128 rows
   constexpr int kQTile = kTileRows * D * 2;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* q_s = smem;
-  unsigned char* ring = smem + 2 * kQTile;
+  unsigned char* ring = smem + NT * kQTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * kStageBytes<D>);
   uint64_t* kv_full = bars;            // [NS] the stage's copies landed
   uint64_t* kv_empty = bars + NS;      // [NS] the MMAs that read the stage are done
@@ -310,22 +323,22 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   TileWork w;
   // block (tile pair, split): the splits of a pair are neighbours; a last pair of one tile may have fewer
   const int item = blockIdx.x / d.kv_heads, kvh = blockIdx.x % d.kv_heads;
-  const int pairs_full = pass.rest ? (d.n_tokens * p.group) / kPairRows : 0x7fffffff;
+  const int pairs_full = pass.rest ? (d.n_tokens * p.group) / (NT * kTileRows) : 0x7fffffff;
   const bool in_rest = item / pass.splits >= pairs_full;
   const int splits = in_rest ? pass.rest : pass.splits;
   const int tile_pair = in_rest ? pairs_full : item / pass.splits;
   const int split = in_rest ? item - pairs_full * pass.splits : item - tile_pair * pass.splits;
-  if (!find_work(p, pass, tile_pair, lane, &w)) return;  // the same for every thread
+  if (!find_work<NT * kTileRows>(p, pass, tile_pair, lane, &w)) return;  // the same for every thread
   const int tiles0 = (w.seg0 + kTileKeys - 1) / kTileKeys, all = tiles0 + (w.seg1 + kTileKeys - 1) / kTileKeys;
   const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
   const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - t0;
-  const int active = w.rows - w.row0 > kTileRows ? 2 : 1;
+  const int active = NT == 2 && w.rows - w.row0 > kTileRows ? 2 : 1;
 
   uint32_t tmem = 0;
-  if (warp != kWarpTma) {
+  if (warp < kWarpTma) {
     if (warp == kWarpPv) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                   :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+                   :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols<D>) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (warp < kWarpQk) {
       // Q into shared memory (128-byte swizzle), rows past the last as zeros; K's first tiles are on their way meanwhile
@@ -350,15 +363,17 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     tc_fence_before();
-    asm volatile("barrier.cta.sync 1, %0;" :: "n"(kThreads - 32) : "memory");
+    asm volatile("barrier.cta.sync 1, %0;" :: "n"(kWarpTma * 32) : "memory");
     tc_fence_after();
     tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   }
   // columns: the scores of either tile, tile t's weights, its output
   const uint32_t s_col = tmem;
   auto p_col = [&](int t) { return tmem + kTileKeys + t * (kTileKeys / 2); };
-  auto o_col = [&](int t) { return tmem + 2 * kTileKeys + t * D; };
+  auto o_col = [&](int t) { return tmem + kTileKeys + NT * (kTileKeys / 2) + t * D; };
 
+  if (warp >= kWarpQk) {
+  if constexpr (NT == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOther));
   if (warp == kWarpTma) {
     // ---------------- K and V tiles: a lane loads a page
     const int box = min(d.page_size, kTileKeys);
@@ -411,7 +426,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       ok = mbar_wait(&kv_full[st], phase, abort_flag);
       const uint64_t b = k0 + static_cast<uint32_t>(st) * (kStageBytes<D> >> 4);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < NT; ++t) {
         if (t == 1 && active < 2) break;
         // the score tile is free once the scores before are in registers
         if (t == 1) ok = ok && mbar_wait(&s_read[0], i & 1, abort_flag);
@@ -455,7 +470,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       ok = mbar_wait(&kv_full[st], phase, abort_flag);
       const uint64_t b = v0 + static_cast<uint32_t>(st) * (kStageBytes<D> >> 4);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < NT; ++t) {
         if (t == 1 && active < 2) break;
         ok = ok && mbar_wait(&p_full[t], i & 1, abort_flag);
         tc_fence_after();
@@ -485,8 +500,10 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       mbar_drain(&mma_done[1], 0);
     }
     __syncwarp();
+  }
   } else {
     // ---------------- softmax: a thread a row
+    if constexpr (NT == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegsSoftmax));
     const int t = warp >> 2;
     if (t < active) {
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -646,14 +663,14 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   tc_fence_before();
   __syncthreads();
   if (warp == kWarpPv)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(kTmemCols<D>) : "memory");
 }
 
 template <int D, bool BF16>
 vqb_status launch(const AttnParams& p, const AttnPass& pass, int64_t tiles, const CUtensorMap& km, const CUtensorMap& vm,
                   cudaStream_t s) {
   constexpr size_t smem = tiles_smem<D>();
-  static_assert(smem <= 232448, "over the opt-in shared memory of an SM");
+  static_assert((D == 128 ? 1 : 2) * (smem + 1024) <= 233472, "over the opt-in shared memory of an SM");
   if (cudaFuncSetAttribute(attention_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
@@ -662,7 +679,7 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, int64_t tiles, cons
                                   : static_cast<int64_t>(tiles) * pass.splits;
   if (items * p.d.kv_heads > 0x7fffffff) return VQB_UNSUPPORTED_GEOMETRY;
   const dim3 grid(static_cast<unsigned>(items * p.d.kv_heads));
-  if (launch_pdl(attention_tiles_kernel<D, BF16>, grid, kThreads, smem, s, p, pass, km, vm) != cudaSuccess)
+  if (launch_pdl(attention_tiles_kernel<D, BF16>, grid, kThreads<D>, smem, s, p, pass, km, vm) != cudaSuccess)
     return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
