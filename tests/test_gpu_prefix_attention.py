@@ -221,6 +221,19 @@ def test_padding_rows_and_strides():
     assert bool((out[n:] == 7).all()) and bool((out[:, 0] == 7).all()) and bool((out[:, 9] == 7).all())
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R,q_len,length,page", [(74, 5, 2200, 128), (90, 9, 700, 16), (160, 5, 390, 64), (40, 70, 1500, 256)])
+def test_few_rows_over_many_keys_each(R, q_len, length, page, D, dtype):
+    """More blocks than SMs, each with little work a key tile: copies of keys and values land late and out of order."""
+    rng = np.random.default_rng(R)
+    lens = rng.integers(length // 2, length, R, endpoint=True).tolist()
+    c = Case([q_len] * R, lens, 0, 16, 4, D, page, dtype, seed=R)
+    first = c.check()
+    for _ in range(20):
+        assert torch.equal(first, c.run())
+
+
 def test_same_result_every_time():
     for q_lens, kv in (([1] * 30, [777] * 30), ([100, 300], [200, 300])):
         c = Case(q_lens, kv, 1500, 10, 2, 128, 64, BF, seed=10)

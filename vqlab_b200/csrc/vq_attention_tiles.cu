@@ -53,11 +53,16 @@ constexpr int kRegsSoftmax = 200, kRegsOther = 56;
 constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial
 template <int D>
 constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
-template <int D>
-constexpr int kStages = 5;
+// Stages of the ring, of K and V tiles in turn.  Even: K and V then have stages of their own, and each stage's "full"
+// barrier one issuer that waits for every one of its phases.  With an odd number a stage holds K and V in turn, each
+// issuer waits for every second phase only, and a wait by parity takes the phase two before its own for its own
+// when the copy between has not landed yet.  Four keep the MMAs as busy as five did (464 us of a 4096-token chunk either
+// way) and leave room for two blocks an SM at D = 64.
+constexpr int kStages = 4;
+static_assert(kStages % 2 == 0, "a stage must hold K tiles only or V tiles only");
 template <int D>
 constexpr size_t tiles_smem() {
-  return 1024 + size_t(kRowTiles<D>) * kTileRows * D * 2 + size_t(kStages<D>) * kStageBytes<D> + 256;
+  return 1024 + size_t(kRowTiles<D>) * kTileRows * D * 2 + size_t(kStages) * kStageBytes<D> + 256;
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -280,7 +285,7 @@ __global__ void __launch_bounds__(kThreads<D>, D == 128 ? 1 : 2)
 attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char smem_raw[];
-  constexpr int NS = kStages<D>, NT = kRowTiles<D>;
+  constexpr int NS = kStages, NT = kRowTiles<D>;
   constexpr int kWarpQk = kSoftmaxWarps<D>, kWarpPv = kWarpQk + 1, kWarpTma = kWarpQk + 2;
   constexpr int kHalf = kTileKeys * 128;  // 64 elements of 128 rows
   constexpr int kQTile = kTileRows * D * 2;
