@@ -405,7 +405,8 @@ vqb_status vqb_ep_reduce(const vqb_ep_layout* layout, void* region, void* y, vqb
  * back go to the ring's end in the order of requests and of their pages, then
  * requests take what they lack from its start in the order of requests.  A
  * request that needs more pages than its row has places, or than are left at
- * its turn (the needs of all before it counted), is refused: its row and its
+ * its turn (the needs of all before it counted), or whose length would pass
+ * 2^31 - 1, is refused: its row and its
  * length stay, its new tokens get slot -1, and so does every later one that
  * lacks a page.
  *

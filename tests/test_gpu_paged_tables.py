@@ -126,6 +126,22 @@ def test_lengths_of_zero_and_no_tokens():
     check(make(2, 4, 16, [0, 0], [64, 0], 4, 11), 16, 64)
 
 
+@pytest.mark.parametrize("page", [2**30, 2**31 - 1, 715827883])
+def test_a_length_past_31_bits_is_refused(page):
+    """The pages would fit the rows; the lengths no longer fit their type.  Requests up to 2^31 - 1 tokens are served."""
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    context, new = [2**31 - 10, 2**31 - 10, 5, 2**31 - 1], [100, 9, 1, 0]
+    held = [-(-c // page) for c in context]
+    table = [[4 * r + j if j < n else -1 for j in range(4)] for r, n in enumerate(held)]
+    out = paged_tables(i32(context), i32(new), i32(table), i32([90, 91, 92, 93]), torch.tensor([0, 4, 0, 0], device="cuda"),
+                       page_size=page, max_tokens=112)
+    assert out.kv_lens.tolist() == [2**31 - 10, 2**31 - 1, 6, 2**31 - 1]
+    assert out.state.tolist() == [0, 4, 1, 0]
+    assert out.block_table.tolist() == table
+    assert out.requests.tolist() == [0] * 100 + [1] * 9 + [2, -1, -1]
+    assert out.slots[:100].tolist() == [-1] * 100
+
+
 def test_more_tokens_than_places_is_safe():
     """Tokens past max_tokens have no place; everything else is as it would be."""
     check(make(3, 8, 16, [3, 0, 20], [30, 10, 7], 9, 12), 16, 20)
