@@ -179,6 +179,21 @@ def test_shared_prefix_batches(R, prefix, context):
     Case([2] * R, rng.integers(2, context + 2, R).tolist(), prefix, 8, 2, 64, 16, FP, seed=R).check()
 
 
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("prefix", [0, 1, 15, 17, 31, 33, 47, 1000])
+def test_ends_inside_a_stage(prefix, page):
+    """Lengths of keys around the 16 and 32 of a stage, the prefix's end and the request's own."""
+    for length in (0, 1, 15, 16, 17, 31, 32, 33, 49, 500):
+        Case([1], [length], prefix, 8, 2, 64, page, FP, seed=prefix + length).check()
+        Case([min(length, 3)], [length], prefix, 8, 2, 128, page, BF, seed=prefix + length).check()
+
+
+@pytest.mark.parametrize("R,KH,length", [(16, 8, 2000), (13, 8, 2000), (74, 8, 300), (74, 8, 450), (150, 4, 300), (40, 8, 2000)])
+def test_small_heads_in_one_round_and_in_several(R, KH, length):
+    rng = np.random.default_rng(R)
+    Case([1] * R, rng.integers(1, length, R, endpoint=True).tolist(), 0, 2 * KH, KH, 64, 32, BF, seed=R).check()
+
+
 def test_long_context_splits():
     """One request over tens of thousands of tokens (split and joined), ragged beside short ones."""
     Case([1], [40001], 0, 8, 2, 128, 64, BF, seed=1).check()

@@ -117,6 +117,12 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
       const int64_t fill = ceil_div(2 * sms, requests_heads * 8), most_k = keys / (8 * 256);
       a.own.splits = static_cast<int>(fill < most_k ? fill : most_k);
     }
+    // At D = 64 stages of 32 keys, which share a stage's fixed work: 24 requests of up to 15000 keys 68 -> 62 us, 250 of up
+    // to 5000 214 -> 205 us.  They leave room for three blocks an SM, stages of 16 for four: where that many are one
+    // round (16 requests of up to 2000 keys in 512 blocks: 11.0 against 13.4 us), or run beside the pass over the
+    // prefix (250 of up to 2500 keys behind 9000: 138 against 142 us), stages have 16.
+    const int64_t n = requests_heads * a.own.cluster * a.own.splits;
+    a.own.stage_keys = d.head_dim == 64 && !joint && !(n > 3 * sms && n <= 4 * sms) ? 32 : 16;
   } else {
     a.own_tiles = rows / block_rows + d.n_requests;
     const int64_t blocks = (rows / block_rows > d.n_requests ? rows / block_rows : d.n_requests) * d.kv_heads;

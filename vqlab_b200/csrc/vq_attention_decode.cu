@@ -24,22 +24,23 @@ namespace vqb {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kUnit = 16;  // keys of a stage
-template <int D>
-constexpr int kStages = D == 128 ? 2 : 3;
-template <int D>
-constexpr int kResident = D == 128 ? 3 : 4;  // blocks an SM: of 64 KB and 168 registers, of 48 KB and 128 registers
-template <int D>
-constexpr int kHalfBytes = kUnit * D * 2;  // K or V of a stage
-template <int D>
-constexpr size_t kRingBytes = size_t(kStages<D>) * 2 * kHalfBytes<D>;  // of a warp; at the end fp32 [16][D]
+constexpr int kGroup = 16;  // keys of a box, which lies in one page
+// A stage holds U keys: 16 at D = 128, 16 or 32 at D = 64 (the plan says when).  Stages of a warp's ring, and blocks an SM: of 64 KB and 168 registers, or of 48 KB and 128 registers.
+template <int D, int U>
+constexpr int kStages = U * D == 1024 ? 3 : 2;
+template <int D, int U>
+constexpr int kResident = U * D == 1024 ? 4 : 3;
+template <int D, int U>
+constexpr int kHalfBytes = U * D * 2;  // K or V of a stage
+template <int D, int U>
+constexpr size_t kRingBytes = size_t(kStages<D, U>) * 2 * kHalfBytes<D, U>;  // of a warp; at the end fp32 [16][D]
 
 // A block's shared memory: the rings first (1024-byte aligned, as the copies'
 // swizzle needs: the block has no other shared memory), then the small things.
-template <int D>
+template <int D, int U>
 struct DecodeSmem {
-  unsigned char rings[kWarps * kRingBytes<D>];
-  uint64_t full[kWarps][kStages<D>];
+  unsigned char rings[kWarps * kRingBytes<D, U>];
+  uint64_t full[kWarps][kStages<D, U>];
   float2 ml[16];  // the block's own
   float m[kWarps][16], l[kWarps][16];
   int abort;
@@ -111,18 +112,18 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, kResident<D>)
+template <int D, bool BF16, int U>
+__global__ void __launch_bounds__(kWarps * 32, kResident<D, U>)
 attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ __align__(1024) unsigned char smem[];
-  DecodeSmem<D>& sm = *reinterpret_cast<DecodeSmem<D>*>(smem);
+  DecodeSmem<D, U>& sm = *reinterpret_cast<DecodeSmem<D, U>*>(smem);
   auto& s_full = sm.full;
   auto& s_m = sm.m;
   auto& s_l = sm.l;
   auto& s_ml = sm.ml;
   int& s_abort = sm.abort;
-  constexpr int NS = kStages<D>;
+  constexpr int NS = kStages<D, U>, kG = U / kGroup, kGroupBytes = kGroup * D * 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const vqb_attention_desc& d = p.d;
   if (threadIdx.x == 0) {
@@ -161,40 +162,45 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
   }
   const int seg0 = pass.prefix ? d.prefix_len : 0;
   const int seg1 = visible(p, rq, rq.nq - 1);
-  const int tiles0 = (seg0 + kUnit - 1) / kUnit, tiles = tiles0 + (seg1 + kUnit - 1) / kUnit;
+  const int tiles0 = (seg0 + U - 1) / U, tiles = tiles0 + (seg1 + U - 1) / U;
   const int split = cluster * ranks + rank, splits = gridDim.x;
   const int u0 = static_cast<int>(static_cast<int64_t>(tiles) * split / splits);
   const int u1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / splits);
   // this warp's groups: u0 + warp, then every fourth
   const int n = u1 - u0 > warp ? (u1 - u0 - warp + kWarps - 1) / kWarps : 0;
-  unsigned char* ring = smem + warp * kRingBytes<D>;
+  unsigned char* ring = smem + warp * kRingBytes<D, U>;
 
-  auto page_of = [&](int k) -> int {  // page of the warp's k-th group
-    if (k >= n) return d.num_pages;
-    const int u = u0 + warp + kWarps * k;
-    const int page = u < tiles0 ? __ldg(p.prefix_pages + ((u * kUnit) >> p.page_shift))
-                                : __ldg(p.table + static_cast<int64_t>(r) * d.table_width +
-                                        (((u - tiles0) * kUnit) >> p.page_shift));
-    return static_cast<unsigned>(page) < static_cast<unsigned>(d.num_pages) ? page : d.num_pages;  // past the end: zeros
+  auto page_of = [&](int k) -> int {  // page of the warp's k-th group of 16 keys (past the end: read as zeros)
+    const int u = u0 + warp + kWarps * (k / kG);
+    const bool own = u >= tiles0;
+    const int key = (own ? u - tiles0 : u) * U + (k % kG) * kGroup;
+    if (k >= n * kG || key >= (own ? seg1 : seg0)) return d.num_pages;
+    const int page = own ? __ldg(p.table + static_cast<int64_t>(r) * d.table_width + (key >> p.page_shift))
+                         : __ldg(p.prefix_pages + (key >> p.page_shift));
+    return static_cast<unsigned>(page) < static_cast<unsigned>(d.num_pages) ? page : d.num_pages;
   };
-  auto issue = [&](int k, int page) {  // one lane
+  // the warp's k-th stage; lane g copies its g-th group
+  auto issue = [&](int k, int page) {
     const int u = u0 + warp + kWarps * k;
-    const int key = (u < tiles0 ? u : u - tiles0) * kUnit;
+    const int key = (u < tiles0 ? u : u - tiles0) * U + lane * kGroup;
     const int off = key & (d.page_size - 1);
     uint64_t* bar = &s_full[warp][k % NS];
-    unsigned char* dst = ring + (k % NS) * 2 * kHalfBytes<D>;
-    mbar_expect_tx(bar, 2 * kHalfBytes<D>);
+    unsigned char* dst = ring + (k % NS) * 2 * kHalfBytes<D, U> + lane * kGroupBytes;
+    if (lane == 0) mbar_expect_tx(bar, 2 * kHalfBytes<D, U>);
+    if constexpr (kG > 1) __syncwarp();
+    if (lane < kG) {
 #pragma unroll
-    for (int h = 0; h < D / 64; ++h) tma_load_4d(&kmap, bar, dst + h * 2048, h * 64, off, kvh, page);
+      for (int h = 0; h < D / 64; ++h) tma_load_4d(&kmap, bar, dst + h * 2048, h * 64, off, kvh, page);
 #pragma unroll
-    for (int h = 0; h < D / 64; ++h) tma_load_4d(&vmap, bar, dst + kHalfBytes<D> + h * 2048, h * 64, off, kvh, page);
+      for (int h = 0; h < D / 64; ++h) tma_load_4d(&vmap, bar, dst + kHalfBytes<D, U> + h * 2048, h * 64, off, kvh, page);
+    }
   };
 
   // pages of 32 groups at a time, one a lane; the next 32 are fetched while these are used
   int pages = page_of(lane), pages_next = page_of(32 + lane);
   for (int k = 0; k < NS; ++k) {
-    const int pg = __shfl_sync(0xffffffffu, pages, k);
-    if (k < n && lane == 0) issue(k, pg);
+    const int pg = __shfl_sync(0xffffffffu, pages, k * kG + lane % kG);
+    if (k < n) issue(k, pg);
   }
 
   // Q as the first operand: rows lane / 4 and lane / 4 + 8
@@ -233,32 +239,36 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
     }
     const int u = u0 + warp + kWarps * k;
     const bool own = u >= tiles0;
-    const int key = (own ? u - tiles0 : u) * kUnit;
-    const uint32_t kb = smem_u32(ring + (k % NS) * 2 * kHalfBytes<D>), vb = kb + kHalfBytes<D>;
-    const int lim0 = min((own ? vis0 : seg0) - key, kUnit), lim1 = min((own ? vis1 : seg0) - key, kUnit);
-    const int held = min((own ? seg1 : seg0) - key, kUnit);
-    if (held < kUnit) {
+    const int key = (own ? u - tiles0 : u) * U;
+    const uint32_t kb = smem_u32(ring + (k % NS) * 2 * kHalfBytes<D, U>), vb = kb + kHalfBytes<D, U>;
+    const int lim0 = min((own ? vis0 : seg0) - key, U), lim1 = min((own ? vis1 : seg0) - key, U);
+    const int held = min((own ? seg1 : seg0) - key, U);
+    if (held < U) {
       // what lies past the last key may be anything: its weight is 0, its value must be finite
-      unsigned char* v = ring + (k % NS) * 2 * kHalfBytes<D> + kHalfBytes<D>;
-      for (int i = lane; i < (kUnit - held) * (D / 8); i += 32) {
+      unsigned char* v = ring + (k % NS) * 2 * kHalfBytes<D, U> + kHalfBytes<D, U>;
+      for (int i = lane; i < (U - held) * (D / 8); i += 32) {
         const int rr = held + i / (D / 8), c = i % (D / 8);
-        *reinterpret_cast<uint4*>(v + (c >> 3) * 2048 + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(v + (rr / kGroup) * kGroupBytes + (c >> 3) * 2048 + (rr % kGroup) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a copy reuses the stage
       __syncwarp();
     }
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float s[2 * kG][4];
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      uint32_t b[4];
-      const int c = ks * 2 + kchunk;
-      ldsm4(b, kb + (c >> 3) * 2048 + krow * 128 + (((c & 7) ^ (krow & 7)) << 4));
-      mma16816<BF16>(s[0], qf[ks], b[0], b[1]);
-      mma16816<BF16>(s[1], qf[ks], b[2], b[3]);
-    }
-    if (__any_sync(0xffffffffu, lim0 < kUnit || lim1 < kUnit)) {
+    for (int t = 0; t < 2 * kG; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        uint32_t b[4];
+        const int c = ks * 2 + kchunk;
+        ldsm4(b, kb + g * kGroupBytes + (c >> 3) * 2048 + krow * 128 + (((c & 7) ^ (krow & 7)) << 4));
+        mma16816<BF16>(s[2 * g], qf[ks], b[0], b[1]);
+        mma16816<BF16>(s[2 * g + 1], qf[ks], b[2], b[3]);
+      }
+    if (__any_sync(0xffffffffu, lim0 < U || lim1 < U)) {
+#pragma unroll
+      for (int t = 0; t < 2 * kG; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int col = t * 8 + (lane & 3) * 2 + e;
@@ -266,8 +276,12 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
           if (col >= lim1) s[t][2 + e] = -INFINITY;
         }
     }
-    float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-    float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+    float t0 = fmaxf(s[0][0], s[0][1]), t1 = fmaxf(s[0][2], s[0][3]);
+#pragma unroll
+    for (int t = 1; t < 2 * kG; ++t) {
+      t0 = fmaxf(t0, fmaxf(s[t][0], s[t][1]));
+      t1 = fmaxf(t1, fmaxf(s[t][2], s[t][3]));
+    }
     t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
     t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
     t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)) * p.scale_log2;
@@ -289,7 +303,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
     }
     const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < 2 * kG; ++t) {
       s[t][0] = exp2_fast(fmaf(s[t][0], p.scale_log2, -b0));
       s[t][1] = exp2_fast(fmaf(s[t][1], p.scale_log2, -b0));
       s[t][2] = exp2_fast(fmaf(s[t][2], p.scale_log2, -b1));
@@ -297,24 +311,28 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
       l0 += s[t][0] + s[t][1];
       l1 += s[t][2] + s[t][3];
     }
-    const uint32_t pf[4] = {pack16<BF16>(s[0][0], s[0][1]), pack16<BF16>(s[0][2], s[0][3]),
-                            pack16<BF16>(s[1][0], s[1][1]), pack16<BF16>(s[1][2], s[1][3])};
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      uint32_t b[4];
-      const int c = i * 2 + vchunk;
-      ldsm4_t(b, vb + (c >> 3) * 2048 + vrow * 128 + (((c & 7) ^ (vrow & 7)) << 4));
-      mma16816<BF16>(o[2 * i], pf, b[0], b[1]);
-      mma16816<BF16>(o[2 * i + 1], pf, b[2], b[3]);
+    for (int g = 0; g < kG; ++g) {
+      const float(*w)[4] = s + 2 * g;
+      const uint32_t pf[4] = {pack16<BF16>(w[0][0], w[0][1]), pack16<BF16>(w[0][2], w[0][3]),
+                              pack16<BF16>(w[1][0], w[1][1]), pack16<BF16>(w[1][2], w[1][3])};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t b[4];
+        const int c = i * 2 + vchunk;
+        ldsm4_t(b, vb + g * kGroupBytes + (c >> 3) * 2048 + vrow * 128 + (((c & 7) ^ (vrow & 7)) << 4));
+        mma16816<BF16>(o[2 * i], pf, b[0], b[1]);
+        mma16816<BF16>(o[2 * i + 1], pf, b[2], b[3]);
+      }
     }
     __syncwarp();
     const int next = k + NS;
-    if ((next & 31) == 0) {
+    if ((next * kG & 31) == 0) {
       pages = pages_next;
-      pages_next = page_of(next + 32 + lane);
+      pages_next = page_of(next * kG + 32 + lane);
     }
-    const int pg = __shfl_sync(0xffffffffu, pages, next & 31);
-    if (next < n && lane == 0) issue(next, pg);
+    const int pg = __shfl_sync(0xffffffffu, pages, (next * kG & 31) + lane % kG);
+    if (next < n) issue(next, pg);
   }
   l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
@@ -338,7 +356,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
   }
   __syncthreads();
   constexpr int kPer = D / 4;  // threads of a row, four elements each
-  constexpr size_t kRing = kRingBytes<D> / sizeof(float);
+  constexpr size_t kRing = kRingBytes<D, U> / sizeof(float);
   float* rings = reinterpret_cast<float*>(smem);
   for (int i = threadIdx.x; i < nrows * kPer; i += kWarps * 32) {
     const int row = i / kPer, e = (i % kPer) * 4;
@@ -389,10 +407,10 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
   if (waits) pdl_wait();
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, int U>
 vqb_status launch(const AttnParams& p, const AttnPass& pass, const AttnPass& shared, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
-  constexpr size_t smem = sizeof(DecodeSmem<D>);
-  if (cudaFuncSetAttribute(attention_decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  constexpr size_t smem = sizeof(DecodeSmem<D, U>);
+  if (cudaFuncSetAttribute(attention_decode_kernel<D, BF16, U>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
   cudaLaunchAttribute attr[2];
@@ -409,7 +427,7 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, const AttnPass& sha
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, attention_decode_kernel<D, BF16>, p, pass, shared, km, vm) != cudaSuccess) return VQB_CUDA_ERROR;
+  if (cudaLaunchKernelEx(&cfg, attention_decode_kernel<D, BF16, U>, p, pass, shared, km, vm) != cudaSuccess) return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
 }
@@ -419,12 +437,13 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, const AttnPass& sha
 vqb_status launch_attention_decode(const AttnParams& p, const AttnPass& pass, const AttnPass& shared, bool bf16, cudaStream_t s) {
   CUtensorMap km, vm;
   const vqb_attention_desc& d = p.d;
-  vqb_status st = encode_pool(&km, d, bf16, p.kc, d.kc_page_stride, d.kc_head_stride, d.kc_token_stride, kUnit);
+  vqb_status st = encode_pool(&km, d, bf16, p.kc, d.kc_page_stride, d.kc_head_stride, d.kc_token_stride, kGroup);
   if (st != VQB_OK) return st;
-  st = encode_pool(&vm, d, bf16, p.vc, d.vc_page_stride, d.vc_head_stride, d.vc_token_stride, kUnit);
+  st = encode_pool(&vm, d, bf16, p.vc, d.vc_page_stride, d.vc_head_stride, d.vc_token_stride, kGroup);
   if (st != VQB_OK) return st;
-  if (d.head_dim == 128) return bf16 ? launch<128, true>(p, pass, shared, km, vm, s) : launch<128, false>(p, pass, shared, km, vm, s);
-  return bf16 ? launch<64, true>(p, pass, shared, km, vm, s) : launch<64, false>(p, pass, shared, km, vm, s);
+  if (d.head_dim == 128) return bf16 ? launch<128, true, 16>(p, pass, shared, km, vm, s) : launch<128, false, 16>(p, pass, shared, km, vm, s);
+  if (pass.stage_keys == 32) return bf16 ? launch<64, true, 32>(p, pass, shared, km, vm, s) : launch<64, false, 32>(p, pass, shared, km, vm, s);
+  return bf16 ? launch<64, true, 16>(p, pass, shared, km, vm, s) : launch<64, false, 16>(p, pass, shared, km, vm, s);
 }
 
 }  // namespace vqb
