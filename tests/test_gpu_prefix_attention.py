@@ -194,6 +194,23 @@ def test_small_heads_in_one_round_and_in_several(R, KH, length):
     Case([1] * R, rng.integers(1, length, R, endpoint=True).tolist(), 0, 2 * KH, KH, 64, 32, BF, seed=R).check()
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R,H,KH,q_len,length,prefix,page", [
+    (64, 40, 8, 5, 200, 0, 16), (90, 10, 2, 4, 90, 0, 64), (150, 20, 4, 6, 40, 333, 32), (64, 17, 1, 1, 500, 0, 16), (200, 4, 4, 32, 60, 0, 16),
+    (40, 24, 8, 7, 64, 1000, 16)])
+def test_between_16_and_32_rows(R, H, KH, q_len, length, prefix, page, D, dtype):
+    """A request's rows in two tiles of 16, the second one full, ragged or empty."""
+    rng = np.random.default_rng(R + q_len)
+    lens = rng.integers(0, length, R, endpoint=True)
+    q_lens = np.minimum(rng.integers(0, q_len, R, endpoint=True), lens)
+    q_lens[0], lens[0] = q_len, length
+    c = Case(q_lens.tolist(), lens.tolist(), prefix, H, KH, D, page, dtype, seed=R)
+    first = c.check()
+    for _ in range(5):
+        assert torch.equal(first, c.run())
+
+
 def test_long_context_splits():
     """One request over tens of thousands of tokens (split and joined), ragged beside short ones."""
     Case([1], [40001], 0, 8, 2, 128, 64, BF, seed=1).check()

@@ -8,7 +8,7 @@
 //   * rows of all requests together over the shared prefix
 //     (vq_attention_tiles.cu): its pages are read once for 256 rows;
 //   * each request's own keys: vq_attention_decode.cu for up to 16 rows a
-//     key/value head, vq_attention_tiles.cu for more;
+//     key/value head (32 in batches of many requests), vq_attention_tiles.cu for more;
 //   * both over splits of the keys where there are fewer blocks than SMs.
 #include "vq_attention.cuh"
 
@@ -33,7 +33,7 @@ constexpr int kMaxSplits = 64;
 
 // Splits of `tiles` key tiles over the tile kernel's blocks: the fewest rounds of
 // the longest block, and the join's traffic (`row_cost`: a partial result's).
-int pick_splits(int64_t blocks, int64_t tiles, int slots, double row_cost, bool joined_anyway) {
+int pick_splits(int64_t blocks, int64_t tiles, int slots, double row_cost, bool joined_anyway, double* time = nullptr) {
   int best = 1;
   double best_t = 1e30;
   for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
@@ -43,6 +43,37 @@ int pick_splits(int64_t blocks, int64_t tiles, int slots, double row_cost, bool 
     if (t < best_t * 0.98) {
       best_t = t;
       best = s;
+    }
+  }
+  if (time) *time = best_t;
+  return best;
+}
+
+// The decode kernel's time with `cluster` blocks a (request, head), in microseconds: what the blocks cost besides their keys,
+// times the rounds (a third of one at least: a block an SM), and their meeting; and the longest run of keys, bound by its own copies, beside all keys, bound by memory (half of the
+// shorter one still shows).  With one row tile a block (two) a round of blocks costs 5 us (10; 7.5 at D = 64) and a key of a
+// run 11.3 ns (25), 0.6 of that at D = 64.  Lengths are taken to average 0.55 of the largest.  Fitted to 32 (14)
+// batches of 1 to 200 requests with 200 to 15000 keys, each timed with 1, 2, 4 and 8 blocks: the choice costs 0.5 % on
+// average against the best of the four.  (Two rounds of blocks with 512 keys or more cost 6 %: 8 requests of up
+// to 900 keys 15.1 us in clusters of 8, 10.3 of 4; 64 of up to 600 28.2 us in clusters of 2, 23.5 without.)
+double decode_time(const vqb_attention_desc& d, int row_tiles, int64_t keys, int cluster, int sms) {
+  const double rh = static_cast<double>(d.n_requests) * d.kv_heads, half = d.head_dim == 64 ? 0.5 : 1.0;
+  const double block = row_tiles == 1 ? 5.0 : d.head_dim == 64 ? 7.5 : 10.0;
+  const double run = static_cast<double>(keys) / cluster * (row_tiles == 1 ? 0.0113 : 0.025) * (d.head_dim == 64 ? 0.6 : 1.0);
+  const double all = 0.55 * keys * rh * 0.08e-3 * half * (row_tiles == 1 ? 1.0 : 1.25);
+  const double rounds = rh * cluster / (3 * sms);
+  const double meet = cluster == 1 ? 0.0 : cluster == 2 ? 0.95 : cluster == 4 ? 1.15 : 1.35;  // the cluster's blocks
+  return meet + block * (rounds > 0.33 ? rounds : 0.33) + (run > all ? run + 0.5 * all : all + 0.5 * run);
+}
+
+int pick_cluster(const vqb_attention_desc& d, int row_tiles, int64_t keys, int sms, double* time) {
+  int best = 1;
+  *time = decode_time(d, row_tiles, keys, 1, sms);
+  for (int c = 2; c <= 8; c *= 2) {
+    const double t = decode_time(d, row_tiles, keys, c, sms);
+    if (t < *time) {
+      *time = t;
+      best = c;
     }
   }
   return best;
@@ -94,7 +125,6 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   const int group = d.heads / d.kv_heads;
   const int64_t rows = static_cast<int64_t>(d.n_tokens) * group;  // of one key/value head
   const int64_t most = static_cast<int64_t>(d.max_q_len < d.n_tokens ? d.max_q_len : d.n_tokens) * group;
-  a.decode = most <= 16;
   // the prefix for all rows at once, unless a request fills tiles by itself
   const bool joint = d.prefix_len > 0 && d.n_requests > 1 && most <= 256;
   // a partial result written and read, at 4 TB/s
@@ -102,19 +132,21 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
   const int64_t requests_heads = static_cast<int64_t>(d.n_requests) * d.kv_heads;
   a.own.prefix = !joint && d.prefix_len > 0;
+  a.own_tiles = rows / block_rows + d.n_requests;
+  const int64_t blocks = (rows / block_rows > d.n_requests ? rows / block_rows : d.n_requests) * d.kv_heads;
+  double tiles_t, decode_t;
+  a.own.splits = pick_splits(blocks, ceil_div(keys, 128), slots, row_cost, joint, &tiles_t);
+  // The decode kernel for up to 16 rows, and for up to 32 where it is the faster one: many requests with few keys leave the
+  // tile kernel's blocks empty (200 requests of 25 rows and up to 300 keys: 61 us, in tiles 105), few requests
+  // with many keep it busy (16 of up to 2000: 36 us, in tiles 29).  With 64 rows a block it had no such batch.
+  a.own.row_tiles = most <= 16 ? 1 : 2;
+  a.own.cluster = pick_cluster(d, a.own.row_tiles, keys, sms, &decode_t);
+  a.decode = most <= 16 || (most <= 32 && decode_t < tiles_t);
   if (a.decode) {
-    // About two rounds of three blocks an SM, so that ragged lengths even out, each
-    // with 512 keys or more (128 where that leaves SMs idle): up to 8 blocks a
-    // (request, head) in a cluster, and several clusters only where 8 would leave
-    // SMs idle.
-    int64_t s = ceil_div(6 * sms, requests_heads);
-    const int64_t most_s = ceil_div(keys, requests_heads * ceil_div(keys, 512) < sms ? 128 : 512);
-    if (s > most_s) s = most_s;
-    a.own.cluster = 1;
-    while (a.own.cluster < 8 && a.own.cluster * 2 <= s) a.own.cluster *= 2;
     a.own.splits = 1;
-    if (requests_heads * 8 < sms && keys > 8 * 512) {  // a join kernel pays from about 500 keys a block on
+    if (most <= 16 && requests_heads * 8 < sms && keys > 8 * 512) {  // a join kernel pays from about 500 keys a block on
       const int64_t fill = ceil_div(2 * sms, requests_heads * 8), most_k = keys / (8 * 256);
+      a.own.cluster = 8;
       a.own.splits = static_cast<int>(fill < most_k ? fill : most_k);
     }
     // At D = 64 stages of 32 keys, which share a stage's fixed work: 24 requests of up to 15000 keys 68 -> 62 us, 250 of up
@@ -123,10 +155,6 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
     // prefix (250 of up to 2500 keys behind 9000: 138 against 142 us), stages have 16.
     const int64_t n = requests_heads * a.own.cluster * a.own.splits;
     a.own.stage_keys = d.head_dim == 64 && !joint && !(n > 3 * sms && n <= 4 * sms) ? 32 : 16;
-  } else {
-    a.own_tiles = rows / block_rows + d.n_requests;
-    const int64_t blocks = (rows / block_rows > d.n_requests ? rows / block_rows : d.n_requests) * d.kv_heads;
-    a.own.splits = pick_splits(blocks, ceil_div(keys, 128), slots, row_cost, joint);
   }
   bool together = !a.decode;  // the own pass leaves partial results too
   if (joint) {

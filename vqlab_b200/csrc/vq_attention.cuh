@@ -38,6 +38,7 @@ struct AttnPass {
   int part0;     // first partial result of the pass, one a split; -1: the pass writes out itself
   int cluster;   // decode kernel: blocks of a cluster, which share a split's keys
   int stage_keys;  // decode kernel: keys of a stage, 16 or 32 (D = 64 only)
+  int row_tiles;   // decode kernel: 16 rows each, of a block (1, 2)
   int first;     // the call's first pass: its first block clears the status block
 };
 
