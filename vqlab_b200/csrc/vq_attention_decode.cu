@@ -9,8 +9,8 @@
 // S = Q K^T and O += P V with m16n8k16 MMAs: Q and O stay in registers, P goes from
 // the accumulator's layout straight into the next MMA's operand.  Of 17 to 32 rows
 // two warps take 16 each and share a ring, whose stages are refilled once both have
-// read them.  Long runs of keys at D = 128 move at 6.6 TB/s (24 requests of up to 15000 keys
-// and 5 rows: 112 us); with two row tiles the MMAs begin to bind (24 of up to 8000 and 20 rows: 106 us, 3.6 TB/s).
+// read them.  Long runs of keys move at 6.1 TB/s at D = 128 (24 requests of up to 15000 keys
+// and 5 rows: 112 us); with two row tiles the MMAs begin to bind (24 of up to 8000 and 20 rows: 106 us, 3.7 TB/s).
 //
 // The results are joined without leaving the kernel: the four warps' in shared
 // memory, then the cluster's over distributed shared memory (each block joins its

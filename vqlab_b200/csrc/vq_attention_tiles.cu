@@ -12,7 +12,7 @@
 //     another O_t += P_t V with P_t in tensor memory and V read along its other
 //     dimension.  Issuing keeps step with the tensor cores, so one thread for both
 //     left them idle while it went from one barrier to the next (3400 cycles a
-//     key tile);
+//     key tile of two row tiles; now 2700);
 //   * four softmax warps a tile, a thread a row: the row's 128 scores into
 //     registers, running maximum and sum, weights as 16-bit numbers to tensor
 //     memory.  O is rescaled in place, by the same thread, only when the maximum
@@ -23,6 +23,8 @@
 // exponentials and no score waits for a P V.  (With a score tile each, weights
 // had to lie over scores, and each tile's chain of exponentials, P V and Q K^T was
 // serial: 3900 cycles a key tile against 2100 of MMAs.)
+// Bound: the MMAs, at the clock that the power cap leaves: 4096 tokens over up to 8192 keys (40 heads, D = 128) take
+// 463 us, 1.11 PFLOP/s; at D = 64 the exponentials, which take longer than a key tile's MMAs.
 // Scores, weights' sum and O are fp32; the weights are rounded once to the
 // cache's type, which the MMA needs.
 //

@@ -9,7 +9,8 @@
 // Bound: bytes (each of q, k, v read once and written once).  A block takes a few
 // tokens: it computes their rotary_dim / 2 sines and cosines once into shared
 // memory, then streams all heads, a thread moving VEC pairs (two 16-byte loads
-// and stores when the layout allows).
+// and stores when the layout allows).  16385 tokens of 40 + 8 + 8 heads of 128:
+// 80 us, 5.9 TB/s; one token 1.9 us in a captured graph.
 #include "vqb_common.cuh"
 #include "vqb_internal.h"
 
