@@ -211,6 +211,22 @@ def test_between_16_and_32_rows(R, H, KH, q_len, length, prefix, page, D, dtype)
         assert torch.equal(first, c.run())
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("R,H,KH,q_len,length,prefix,page", [
+    (60, 24, 3, 16, 600, 0, 16), (40, 20, 4, 25, 300, 200, 64), (75, 4, 2, 64, 129, 0, 32), (160, 35, 1, 3, 1000, 0, 128), (20, 16, 8, 33, 2000, 0, 16)])
+def test_one_tile_of_rows_each(R, H, KH, q_len, length, prefix, page, causal, dtype):
+    """More (request, head)s than SMs, each with up to 128 rows: none, a few, a whole tile; keys from none to many tiles."""
+    rng = np.random.default_rng(R + q_len)
+    lens = rng.integers(0, length, R, endpoint=True)
+    q_lens = np.minimum(rng.integers(0, q_len, R, endpoint=True), lens)
+    q_lens[0], lens[0] = q_len, length
+    c = Case(q_lens.tolist(), lens.tolist(), prefix, H, KH, 128, page, dtype, seed=R)
+    first = c.check(causal=causal)
+    for _ in range(5):
+        assert torch.equal(first, c.run(causal=causal))
+
+
 def test_long_context_splits():
     """One request over tens of thousands of tokens (split and joined), ragged beside short ones."""
     Case([1], [40001], 0, 8, 2, 128, 64, BF, seed=1).check()

@@ -132,16 +132,22 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   const int64_t keys = static_cast<int64_t>(d.max_kv_len) + (joint ? 0 : d.prefix_len);
   const int64_t requests_heads = static_cast<int64_t>(d.n_requests) * d.kv_heads;
   a.own.prefix = !joint && d.prefix_len > 0;
-  a.own_tiles = rows / block_rows + d.n_requests;
-  const int64_t blocks = (rows / block_rows > d.n_requests ? rows / block_rows : d.n_requests) * d.kv_heads;
+  // A request's own rows at D = 128: blocks of two row tiles, or, where requests have one tile and are more than SMs, blocks of
+  // one, two an SM (86 requests of 40 rows and up to 64 keys 39 -> 27 us, 24 of 20 rows and up to 8000 keys 106 -> 95 us; 16
+  // of 25 rows and up to 2000 keys on 128 blocks would take 32 us instead of 29).
+  const int own_rows = d.head_dim == 128 && (most > 128 || requests_heads <= sms) ? 256 : 128;
+  a.own_tiles = rows / own_rows + d.n_requests;
+  const int64_t blocks = (rows / own_rows > d.n_requests ? rows / own_rows : d.n_requests) * d.kv_heads;
   double tiles_t, decode_t;
-  a.own.splits = pick_splits(blocks, ceil_div(keys, 128), slots, row_cost, joint, &tiles_t);
-  // The decode kernel for up to 16 rows, and for up to 32 where it is the faster one: many requests with few keys leave the
-  // tile kernel's blocks empty (200 requests of 25 rows and up to 300 keys: 61 us, in tiles 105), few requests
-  // with many keep it busy (16 of up to 2000: 36 us, in tiles 29).  With 64 rows a block it had no such batch.
-  a.own.row_tiles = most <= 16 ? 1 : 2;
-  a.own.cluster = pick_cluster(d, a.own.row_tiles, keys, sms, &decode_t);
+  a.own.splits = pick_splits(blocks, ceil_div(keys, 128), own_rows == 256 ? sms : 2 * sms, row_cost, joint, &tiles_t);
+  // The decode kernel for up to 16 rows, and for up to 32 where it is the faster one: short contexts, and D = 64 (200 requests of
+  // 25 rows and up to 300 keys 60 us, in tiles 73; 64 of 25 rows at D = 64 and up to 1000 keys 27 us, in tiles 32; but 64 of 25
+  // rows and up to 2500 keys 91 us, in tiles 86, and 16 of up to 500 17 us, in tiles 13).  With 64 rows a block the tile kernel
+  // had nearly every batch.
+  const int decode_tiles = most <= 16 ? 1 : 2;
+  a.own.cluster = pick_cluster(d, decode_tiles, keys, sms, &decode_t);
   a.decode = most <= 16 || (most <= 32 && decode_t < tiles_t);
+  a.own.row_tiles = a.decode ? decode_tiles : own_rows / 128;
   if (a.decode) {
     a.own.splits = 1;
     if (most <= 16 && requests_heads * 8 < sms && keys > 8 * 512) {  // a join kernel pays from about 500 keys a block on
@@ -159,6 +165,7 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   bool together = !a.decode;  // the own pass leaves partial results too
   if (joint) {
     a.shared.joint = 1;
+    a.shared.row_tiles = block_rows / 128;
     a.shared.first = 1;
     a.shared_tiles = ceil_div(rows, block_rows);
     // the last block has one row tile with rows, of two

@@ -38,11 +38,11 @@ struct AttnPass {
   int part0;     // first partial result of the pass, one a split; -1: the pass writes out itself
   int cluster;   // decode kernel: blocks of a cluster, which share a split's keys
   int stage_keys;  // decode kernel: keys of a stage, 16 or 32 (D = 64 only)
-  int row_tiles;   // decode kernel: 16 rows each, of a block (1, 2)
+  int row_tiles;   // of a block: 16 rows each (decode kernel) or 128 (tile kernel), one or two
   int first;     // the call's first pass: its first block clears the status block
 };
 
-// Rows of a key/value head that one block of the tile kernel takes.
+// Rows of a key/value head that one block of the tile kernel takes in the pass over the prefix.
 __host__ __device__ constexpr int tile_block_rows(int head_dim) { return head_dim == 128 ? 256 : 128; }
 
 // Partial results of the pass over the prefix that a row has: `row` counts the

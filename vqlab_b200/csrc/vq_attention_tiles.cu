@@ -3,9 +3,9 @@
 // prefix that it shares (each prefix page is then read once for 256 rows
 // instead of once a request).
 //
-// A block takes (256 rows of one key/value head, 128 at D = 64, and a run of keys): two tiles of
+// A block takes (256 rows of one key/value head and a run of keys): two tiles of
 // 128 rows (a row = a token and a head of the group) that share every K and V
-// tile of 128 keys.  Roles:
+// tile of 128 keys; or, at D = 64 and for requests of up to 128 rows, one tile.  Roles:
 //   * a TMA warp fills a ring of shared-memory stages with K and V tiles, one
 //     box a page and 64 elements (a lane a page);
 //   * one thread issues S = Q_t K^T (both from shared memory) into tensor memory,
@@ -17,7 +17,7 @@
 //     registers, running maximum and sum, weights as 16-bit numbers to tensor
 //     memory.  O is rescaled in place, by the same thread, only when the maximum
 //     has grown by more than 2^kSlack.
-// Tensor memory's 512 columns (at D = 128) hold two O tiles (256), two weight tiles
+// Tensor memory's 512 columns (two tiles, D = 128) hold two O tiles (256), two weight tiles
 // (128) and one score tile (128) that the two row tiles use in turn: it is free again as
 // soon as the scores are in registers, so the next Q K^T runs beside this tile's
 // exponentials and no score waits for a P V.  (With a score tile each, weights
@@ -37,19 +37,16 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-// Row tiles of a block: two at D = 128; one at D = 64, where two blocks share an SM
-// (tensor memory then holds 256 columns of each): their starts and ends overlap, and rows
-// are dealt in 128s.
-template <int D>
-constexpr int kRowTiles = tile_block_rows(D) / kTileRows;
-// four softmax warps a row tile, then one each for Q K^T, P V and the copies
-template <int D>
-constexpr int kSoftmaxWarps = 4 * kRowTiles<D>;
-template <int D>
-constexpr int kThreads = D == 128 ? 352 : 256;
-template <int D>
-constexpr int kTmemCols = D == 128 ? 512 : 256;
-// Registers a thread at D = 64: 256 x 128 at launch; the last four warps leave 72 each,
+// NT row tiles a block.  Two (D = 128): one block an SM.  One (D = 64, and at D = 128 requests of up to 128 rows): two
+// blocks share an SM, 256 columns of tensor memory each, so that their starts and ends overlap and rows are dealt in 128s.
+// At D = 128 a tile's weights then lie over its scores, the next Q K^T waits for P V, and the other block fills the gaps.
+template <int NT>
+constexpr int kSoftmaxWarps = 4 * NT;  // four a row tile; then a warp each for Q K^T, P V and the copies
+template <int NT>
+constexpr int kThreads = NT == 2 ? 352 : 256;
+template <int NT>
+constexpr int kTmemCols = NT == 2 ? 512 : 256;
+// Registers a thread with one row tile: 256 x 128 at launch; the last four warps leave 72 each,
 // which the softmax warps take: 128 x 200 + 128 x 56.
 constexpr int kRegsSoftmax = 200, kRegsOther = 56;
 constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial
@@ -60,11 +57,11 @@ constexpr int kStageBytes = kTileKeys * D * 2;  // a K or a V tile
 // issuer waits for every second phase only, and a wait by parity takes the phase two before its own for its own
 // when the copy between has not landed yet.  Four keep the MMAs as busy as five did (464 us of a 4096-token chunk either
 // way) and leave room for two blocks an SM at D = 64.
-constexpr int kStages = 4;
-static_assert(kStages % 2 == 0, "a stage must hold K tiles only or V tiles only");
-template <int D>
+template <int D, int NT>
+constexpr int kStages = D == 128 && NT == 1 ? 2 : 4;
+template <int D, int NT>
 constexpr size_t tiles_smem() {
-  return 1024 + size_t(kRowTiles<D>) * kTileRows * D * 2 + size_t(kStages) * kStageBytes<D> + 256;
+  return 1024 + size_t(NT) * kTileRows * D * 2 + size_t(kStages<D, NT>) * kStageBytes<D> + 256;
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -282,13 +279,15 @@ __device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& p
   return false;
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads<D>, D == 128 ? 1 : 2)
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(kThreads<NT>, NT == 2 ? 1 : 2)
 attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char smem_raw[];
-  constexpr int NS = kStages, NT = kRowTiles<D>;
-  constexpr int kWarpQk = kSoftmaxWarps<D>, kWarpPv = kWarpQk + 1, kWarpTma = kWarpQk + 2;
+  constexpr int NS = kStages<D, NT>;
+  static_assert(NS % 2 == 0, "a stage must hold K tiles only or V tiles only");
+  constexpr bool kOver = D == 128 && NT == 1;  // weights over scores
+  constexpr int kWarpQk = kSoftmaxWarps<NT>, kWarpPv = kWarpQk + 1, kWarpTma = kWarpQk + 2;
   constexpr int kHalf = kTileKeys * 128;  // 64 elements of 128 rows
   constexpr int kQTile = kTileRows * D * 2;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -345,7 +344,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   if (warp < kWarpTma) {
     if (warp == kWarpPv) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                   :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols<D>) : "memory");
+                   :: "r"(smem_u32(tmem_slot)), "r"(kTmemCols<NT>) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (warp < kWarpQk) {
       // Q into shared memory (128-byte swizzle), rows past the last as zeros; K's first tiles are on their way meanwhile
@@ -376,8 +375,8 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   }
   // columns: the scores of either tile, tile t's weights, its output
   const uint32_t s_col = tmem;
-  auto p_col = [&](int t) { return tmem + kTileKeys + t * (kTileKeys / 2); };
-  auto o_col = [&](int t) { return tmem + kTileKeys + NT * (kTileKeys / 2) + t * D; };
+  auto p_col = [&](int t) { return kOver ? tmem : tmem + kTileKeys + t * (kTileKeys / 2); };
+  auto o_col = [&](int t) { return tmem + kTileKeys + (kOver ? 0 : NT * (kTileKeys / 2)) + t * D; };
 
   if (warp >= kWarpQk) {
   if constexpr (NT == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegsOther));
@@ -435,9 +434,9 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (t == 1 && active < 2) break;
-        // the score tile is free once the scores before are in registers
+        // the score tile is free once the scores before are in registers (kOver: once their weights have met the values)
         if (t == 1) ok = ok && mbar_wait(&s_read[0], i & 1, abort_flag);
-        else if (i > 0) ok = ok && mbar_wait(&s_read[active - 1], (i - 1) & 1, abort_flag);
+        else if (i > 0) ok = ok && mbar_wait(kOver ? &o_full[0] : &s_read[active - 1], (i - 1) & 1, abort_flag);
         tc_fence_after();
         __syncwarp();
         if (issuer && ok) {
@@ -670,15 +669,15 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
   tc_fence_before();
   __syncthreads();
   if (warp == kWarpPv)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(kTmemCols<D>) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(kTmemCols<NT>) : "memory");
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, int NT>
 vqb_status launch(const AttnParams& p, const AttnPass& pass, int64_t tiles, const CUtensorMap& km, const CUtensorMap& vm,
                   cudaStream_t s) {
-  constexpr size_t smem = tiles_smem<D>();
-  static_assert((D == 128 ? 1 : 2) * (smem + 1024) <= 233472, "over the opt-in shared memory of an SM");
-  if (cudaFuncSetAttribute(attention_tiles_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  constexpr size_t smem = tiles_smem<D, NT>();
+  static_assert((NT == 2 ? 1 : 2) * (smem + 1024) <= 233472, "over the opt-in shared memory of an SM");
+  if (cudaFuncSetAttribute(attention_tiles_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return VQB_CUDA_ERROR;
   // the rows with the most keys first, over all heads
@@ -686,7 +685,7 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, int64_t tiles, cons
                                   : static_cast<int64_t>(tiles) * pass.splits;
   if (items * p.d.kv_heads > 0x7fffffff) return VQB_UNSUPPORTED_GEOMETRY;
   const dim3 grid(static_cast<unsigned>(items * p.d.kv_heads));
-  if (launch_pdl(attention_tiles_kernel<D, BF16>, grid, kThreads<D>, smem, s, p, pass, km, vm) != cudaSuccess)
+  if (launch_pdl(attention_tiles_kernel<D, BF16, NT>, grid, kThreads<NT>, smem, s, p, pass, km, vm) != cudaSuccess)
     return VQB_CUDA_ERROR;
   note_launch();
   return VQB_OK;
@@ -694,7 +693,7 @@ vqb_status launch(const AttnParams& p, const AttnPass& pass, int64_t tiles, cons
 
 }  // namespace
 
-// tiles: an upper bound of the pairs of row tiles of the pass.
+// tiles: an upper bound of the blocks of rows (pass.row_tiles row tiles each) of the pass.
 vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, bool bf16, int64_t tiles, cudaStream_t s) {
   CUtensorMap km, vm;
   const vqb_attention_desc& d = p.d;
@@ -703,9 +702,11 @@ vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, boo
   if (st != VQB_OK) return st;
   st = encode_pool(&vm, d, bf16, p.vc, d.vc_page_stride, d.vc_head_stride, d.vc_token_stride, box);
   if (st != VQB_OK) return st;
+  if (d.head_dim == 128 && pass.row_tiles == 2)
+    return bf16 ? launch<128, true, 2>(p, pass, tiles, km, vm, s) : launch<128, false, 2>(p, pass, tiles, km, vm, s);
   if (d.head_dim == 128)
-    return bf16 ? launch<128, true>(p, pass, tiles, km, vm, s) : launch<128, false>(p, pass, tiles, km, vm, s);
-  return bf16 ? launch<64, true>(p, pass, tiles, km, vm, s) : launch<64, false>(p, pass, tiles, km, vm, s);
+    return bf16 ? launch<128, true, 1>(p, pass, tiles, km, vm, s) : launch<128, false, 1>(p, pass, tiles, km, vm, s);
+  return bf16 ? launch<64, true, 1>(p, pass, tiles, km, vm, s) : launch<64, false, 1>(p, pass, tiles, km, vm, s);
 }
 
 }  // namespace vqb
