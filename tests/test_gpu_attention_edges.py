@@ -1,0 +1,38 @@
+"""vqb_prefix_attention where few numbers decide: tiny weights beside a large one,
+scores and values that are not finite, bounds below the lengths.
+
+Tolerances are those of test_gpu_prefix_attention.py (derived there, before any run).
+"""
+import pytest
+import torch
+
+from test_gpu_prefix_attention import BF, FP, Case
+
+pytestmark = pytest.mark.gpu
+
+
+def sink(c, gap, place):
+    """One key `gap` nats above all others, which score 0 alike: its values 0, theirs between 0.5 and 1.5.
+    The others' weights are exp(-gap) of its own, and the whole result.  Returns the scale of such a call."""
+    c.q.zero_()
+    c.q[..., 0] = 4.0
+    c.k.copy_(torch.where(torch.isnan(c.k), c.k, 0.0))
+    c.v.copy_(torch.where(torch.isnan(c.v), c.v, 0.5 + c.v.float().abs().clamp(max=2.0) / 2).to(c.dtype))
+    for r in range(len(c.lens)):
+        pages, j = (c.prefix_pages, place) if c.prefix else (c.table[r], place % c.lens[r])
+        p, o = int(pages[j // c.page]), j % c.page
+        c.k[p, :, o, 0] = gap
+        c.v[p, :, o] = 0.0
+    return 0.25
+
+
+# Weights from exp(-17) = 2^-24.5 of the row's largest on take one rounding of u, as the tolerance has it.
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("gap", [10.0, 13.0, 14.25, 16.0, 17.0])
+@pytest.mark.parametrize("R,q_len,length,prefix,H,KH,D,page", [
+    (2, 1, 8192, 0, 8, 2, 64, 32), (20, 1, 5000, 0, 8, 8, 128, 16), (20, 3, 3000, 0, 15, 3, 64, 16),
+    (70, 5, 700, 0, 15, 3, 128, 16), (1, 300, 8200, 0, 8, 2, 64, 128), (1, 300, 8200, 0, 8, 2, 128, 64),
+    (75, 16, 1500, 0, 24, 3, 128, 64), (30, 1, 40, 8192, 10, 2, 128, 64), (30, 1, 40, 8192, 10, 2, 64, 64)])
+def test_small_weights_beside_a_large_one(R, q_len, length, prefix, H, KH, D, page, gap, dtype):
+    c = Case([q_len] * R, [length] * R, prefix, H, KH, D, page, dtype, seed=R + D)
+    c.check(scale=sink(c, gap, 3))

@@ -55,10 +55,19 @@ vqb_status launch_attention_tiles(const AttnParams& p, const AttnPass& pass, boo
 vqb_status launch_attention_decode(const AttnParams& p, const AttnPass& pass, const AttnPass& shared, bool bf16, cudaStream_t s);
 
 constexpr float kLn2 = 0.6931471805599453f;
-// The running maximum follows the scores only when they pass it by this many
-// powers of two: weights stay below 2^8, exact in relative terms in both 16-bit
-// types, and what has been summed is rescaled only a few times in a long row.
-constexpr float kSlack = 8.0f;
+// A weight is 2^(s - m + kLift), m the running maximum, which follows the scores only
+// when they pass it by more than kSlack powers of two: what has been summed is rescaled
+// a few times in a long row.  The weights are rounded to the cache's type, and each has
+// to keep its relative accuracy, since thousands of small ones may be all of a result (one
+// key with a large score and a value of 0 beside them).  bf16 has fp32's exponents.  fp16 is
+// accurate from 2^-14 to 2^16, so its weights are lifted to end below 2^15 and are
+// good down to 2^-25 of the row's largest; below that a weight is off by at most 2^-36 of it.
+// (Without the lift 699 weights of e^-17 came out 44 % too large, of e^-17.5 as 0.)  Partial
+// results and the log-sum-exp carry m - kLift for m.
+template <bool BF16>
+constexpr float kSlack = BF16 ? 8.0f : 4.0f;
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.0f : 11.0f;
 
 template <bool BF16>
 __device__ __forceinline__ uint16_t narrow16(float v) {

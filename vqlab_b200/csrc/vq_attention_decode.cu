@@ -302,7 +302,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
       t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
       t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2)) * p.scale_log2;
       t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2)) * p.scale_log2;
-      if (__any_sync(0xffffffffu, t0 > m0 + kSlack || t1 > m1 + kSlack)) {
+      if (__any_sync(0xffffffffu, t0 > m0 + kSlack<BF16> || t1 > m1 + kSlack<BF16>)) {
         const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
         const float f0 = n0 == -INFINITY ? 1.0f : exp2_fast(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : exp2_fast(m1 - n1);
         m0 = n0;
@@ -317,7 +317,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
           o[i][3] *= f1;
         }
       }
-      const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+      const float b0 = m0 == -INFINITY ? 0.0f : m0 - kLift<BF16>, b1 = m1 == -INFINITY ? 0.0f : m1 - kLift<BF16>;
 #pragma unroll
       for (int t = 0; t < 2 * kG; ++t) {
         s[t][0] = exp2_fast(fmaf(s[t][0], p.scale_log2, -b0));
@@ -379,9 +379,9 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
     *reinterpret_cast<float2*>(mine + row1 * D + e) = make_float2(o[i][2], o[i][3]);
   }
   if ((lane & 3) == 0) {
-    s_m[warp][row0] = m0;
+    s_m[warp][row0] = m0 - kLift<BF16>;
     s_l[warp][row0] = l0;
-    s_m[warp][row1] = m1;
+    s_m[warp][row1] = m1 - kLift<BF16>;
     s_l[warp][row1] = l1;
   }
   __syncthreads();

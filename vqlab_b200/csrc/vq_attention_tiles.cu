@@ -543,7 +543,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         }
         const float mx = max128(s) * p.scale_log2;
         bool fresh = i == 0;
-        if (__any_sync(0xffffffffu, mx > m + kSlack)) {
+        if (__any_sync(0xffffffffu, mx > m + kSlack<BF16>)) {
           const float mn = fmaxf(m, mx);
           const float f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
           m = mn;
@@ -563,7 +563,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
             }
           }
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float base = m == -INFINITY ? 0.0f : m - kLift<BF16>;
         const uint64_t base2 = pair(-base, -base);
         uint32_t pk0[16], pk1[16];
         l += weights32<BF16>(pk0, s, scale2, base2);
@@ -602,6 +602,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
       if (!ok && lane == 0) *p.status = VQB_TIMEOUT;
       if (ok) {
         tc_fence_after();
+        m -= kLift<BF16>;
         const int64_t token = w.rq.q0 + tok;
         const int head = kvh * p.group + (gv - tok * p.group);
         const int64_t grow = token * d.heads + head;
