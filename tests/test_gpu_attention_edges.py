@@ -36,3 +36,20 @@ def sink(c, gap, place):
 def test_small_weights_beside_a_large_one(R, q_len, length, prefix, H, KH, D, page, gap, dtype):
     c = Case([q_len] * R, [length] * R, prefix, H, KH, D, page, dtype, seed=R + D)
     c.check(scale=sink(c, gap, 3))
+
+
+@pytest.mark.parametrize("q_len,prefix", [(3, 60), (3, 0), (40, 0), (40, 130), (300, 60)])
+def test_values_that_are_not_finite_leave_the_log_sum_exp(q_len, prefix):
+    """Scores alone make the log-sum-exp: no value changes it, seen or not, one of a row's or all of them."""
+    for D, page, dtype in ((128, 16, BF), (64, 64, FP)):
+        c = Case([q_len] * 3, [q_len + 200, q_len + 60, q_len], prefix, 4, 2, D, page, dtype, seed=16)
+        want = c.run(return_lse=True)[1]
+        assert torch.isfinite(want).all()
+        v0 = c.v.clone()
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            for r, j in ((0, 0), (0, q_len + 199), (1, q_len + 59), (2, q_len - 1)):
+                c.v.copy_(v0)
+                c.v[int(c.table[r, j // page]), :, j % page] = bad
+                assert torch.equal(c.run(return_lse=True)[1], want), (bad, r, j)
+            c.v.fill_(bad)
+            assert torch.equal(c.run(return_lse=True)[1], want), bad

@@ -264,6 +264,7 @@ __device__ __forceinline__ float widen16(uint16_t h) {
 // A row that is not finite, of a request whose later keys it does not see: worked out
 // again, by a warp, over the keys that it does see -- if one of the values that it
 // does not see is indeed not finite.  A row that is not finite by what it sees stays so.
+// The log-sum-exp stays as the passes wrote it: it has no values in it.
 template <int D, bool BF16>
 __device__ void exact_row(const AttnParams& p, int request, const RequestRows& rq, int64_t token, int head) {
   const vqb_attention_desc& d = p.d;
@@ -293,7 +294,7 @@ __device__ void exact_row(const AttnParams& p, int request, const RequestRows& r
   float acc[D / 32];
   float m = -INFINITY, l = 0.0f;
   for (int e = 0; e < D / 32; ++e) acc[e] = 0.0f;
-  bool nan = false;  // NaN it stays, whatever follows
+  bool nan = false;  // NaN the row stays, whatever follows
   for (int part = 0; part < 2; ++part) {
     const int end = part ? seen : d.prefix_len;
     for (int j0 = 0; j0 < end && !nan; j0 += 32) {
@@ -329,7 +330,6 @@ __device__ void exact_row(const AttnParams& p, int request, const RequestRows& r
   uint16_t* out = p.out + token * d.out_token_stride + head * d.out_head_stride;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   for (int e = 0; e < D / 32; ++e) out[lane + 32 * e] = narrow16<BF16>(acc[e] * inv);
-  if (p.lse && lane == 0) p.lse[token * d.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // After the passes of a call that masks keys: nothing, unless a pass noted a row
