@@ -53,3 +53,39 @@ def test_values_that_are_not_finite_leave_the_log_sum_exp(q_len, prefix):
                 assert torch.equal(c.run(return_lse=True)[1], want), (bad, r, j)
             c.v.fill_(bad)
             assert torch.equal(c.run(return_lse=True)[1], want), bad
+
+
+@pytest.mark.parametrize("q_lens,lens,prefix,H,KH,D", [
+    ([2] * 60, [17] * 60, 0, 16, 8, 64), ([3] * 30, [40] * 30, 700, 15, 3, 128), ([70] * 4, [90] * 4, 0, 4, 2, 128), ([2, 300], [5, 300], 0, 4, 2, 64)])
+def test_notes_of_spoiled_rows_in_one_workspace(q_lens, lens, prefix, H, KH, D):
+    """Whatever a workspace held, however often a captured call replays: a masked value that is not finite leaves no trace."""
+    c = Case(q_lens, lens, prefix, H, KH, D, 16, BF, seed=20)
+    want = c.run()
+    clean = c.v.clone()
+    spoiled = c.v.clone()
+    cu = c.cu.tolist()
+    seen = torch.ones(want.shape[0], dtype=torch.bool, device="cuda")
+    for r, n in enumerate(lens):  # each request's last key: its last query alone sees it
+        spoiled[int(c.table[r, (n - 1) // 16]), :, (n - 1) % 16] = float("inf")
+        seen[cu[r + 1] - 1] = False
+    ws = torch.full((1 << 26,), 255, dtype=torch.uint8, device="cuda")
+
+    def right(got, bad):
+        return torch.equal(got[seen], want[seen]) if not bad else bool(torch.isfinite(got[seen]).all()) and bool(
+            ((got - want).abs() <= 2.0 ** -6 * (want.abs() + 1))[seen].all()) and not bool(torch.isfinite(got[~seen]).any())
+    for fill in (255, 0, 1):
+        ws.fill_(fill)
+        for bad in (True, False, True, True):
+            c.v.copy_(spoiled if bad else clean)
+            assert right(c.run(workspace=ws), bad)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = c.run(workspace=ws)
+    for bad in (True, False, False, True, True, False):
+        c.v.copy_(spoiled if bad else clean)
+        g.replay()
+        torch.cuda.synchronize()
+        assert right(out, bad)
+        assert ws[:20].view(torch.int32).tolist()[1:] == [0, 0, 0, 0]  # no status, no count, no note left

@@ -10,6 +10,8 @@
 //   * each request's own keys: vq_attention_decode.cu for up to 16 rows a
 //     key/value head (32 in batches of many requests), vq_attention_tiles.cu for more;
 //   * both over splits of the keys where there are fewer blocks than SMs.
+#include <atomic>
+
 #include "vq_attention.cuh"
 
 namespace vqb {
@@ -188,7 +190,7 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   return a;
 }
 
-constexpr size_t kStatusBytes = 256;
+constexpr size_t kStatusBytes = 256;  // the status block (16 bytes), then the note
 
 size_t part_rows(const vqb_attention_desc& d) { return static_cast<size_t>(d.n_tokens) * d.heads; }
 size_t ml_bytes(const vqb_attention_desc& d, int parts) { return (parts * part_rows(d) * sizeof(float2) + 255) & ~size_t(255); }
@@ -333,12 +335,13 @@ __device__ void exact_row(const AttnParams& p, int request, const RequestRows& r
 }
 
 // After the passes of a call that masks keys: nothing, unless a pass noted a row
-// that is not finite.
+// that is not finite.  The last block to end takes the note away, since a captured call
+// has one mark for all its replays; status[1], which counts the blocks, was cleared in an earlier launch.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) attention_exact_kernel(AttnParams p) {
   pdl_wait();
   pdl_trigger();
-  if (__ldcg(p.status + 1) == 0) return;
+  if (__ldcg(p.note) != p.mark) return;
   const vqb_attention_desc& d = p.d;
   const int lane = threadIdx.x & 31;
   const int64_t rows = static_cast<int64_t>(min(__ldg(p.cu_q + d.n_requests), d.n_tokens)) * d.heads;
@@ -351,6 +354,11 @@ __global__ void __launch_bounds__(256) attention_exact_kernel(AttnParams p) {
     if (!__any_sync(0xffffffffu, bad)) continue;
     const int r = request_of(p.cu_q, d.n_requests, static_cast<int>(n));
     exact_row<D, BF16>(p, r, request_rows(p, r), n, h);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && atomicAdd(p.status + 1, 1) == static_cast<int>(gridDim.x) - 1) {
+    *p.note = 0;
+    p.status[1] = 0;
   }
 }
 
@@ -438,13 +446,16 @@ extern "C" vqb_status vqb_prefix_attention(const vqb_attention_desc* desc, vqb_d
     return VQB_BAD_ALIGNMENT;
   if (workspace_bytes < vqb_prefix_attention_workspace_size(desc)) return VQB_WORKSPACE_TOO_SMALL;
   const AttnPlan a = make_plan(d, kPlanSms);
+  static std::atomic<uint32_t> calls{0};
+  uint32_t mark = ++calls;
+  if (mark == 0) mark = ++calls;
   const bool bf = dtype == VQB_BF16;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   AttnParams p{d, static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache),
                static_cast<const uint16_t*>(v_cache), block_table, kv_lens, cu_q, prefix_pages,
                static_cast<uint16_t*>(out), lse, reinterpret_cast<float*>(ws + kStatusBytes + ml_bytes(d, a.parts)),
-               reinterpret_cast<float2*>(ws + kStatusBytes), reinterpret_cast<int*>(ws) + 1, d.heads / d.kv_heads,
+               reinterpret_cast<float2*>(ws + kStatusBytes), reinterpret_cast<int*>(ws) + 1, reinterpret_cast<uint32_t*>(ws) + 4, mark, d.heads / d.kv_heads,
                __builtin_ctz(d.page_size), d.scale * 1.4426950408889634f};
   timer_before(s);
   if (a.shared.splits > 0) {

@@ -23,7 +23,9 @@ struct AttnParams {
   float* lse;
   float* part_o;
   float2* part_ml;
-  int* status;      // int32 [1] of the workspace; [2]: a masked value may have spoiled a row
+  int* status;      // int32 [1] of the workspace
+  uint32_t* note;   // behind the status block: `mark` once a masked value may have spoiled a row of this call
+  uint32_t mark;    // this call's, not 0
   int group;
   int page_shift;
   float scale_log2;  // scale * log2(e): scores in powers of two
@@ -89,7 +91,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // The status block starts at zero: written by the call's first block as it starts,
-// 2 s before any wait can give up.
+// 2 s before any wait can give up.  Nothing else of the call's first launch may write
+// there: no order holds between its blocks.
 __device__ __forceinline__ void clear_status(const AttnParams& p, const AttnPass& pass) {
   if (pass.first && (blockIdx.x | blockIdx.y | blockIdx.z) == 0 && threadIdx.x < 4) p.status[static_cast<int>(threadIdx.x) - 1] = 0;
 }
@@ -97,7 +100,10 @@ __device__ __forceinline__ void clear_status(const AttnParams& p, const AttnPass
 // The MMAs multiply a masked value by a weight of 0, which is NaN where the value is
 // not finite.  A pass that masks keys says here that a row of it came out not
 // finite; a kernel after the passes then works such rows out again (vq_attention.cu).
-__device__ __forceinline__ void note_not_finite(const AttnParams& p) { p.status[1] = 1; }
+// The note is the call's own mark, so that no one has to clear it before: whatever
+// the word held, it says nothing of this call.  (A word that the first block sets to 0
+// could lose another block's note.)
+__device__ __forceinline__ void note_not_finite(const AttnParams& p) { *p.note = p.mark; }
 
 // The queries of request r, as far as the call's bounds go.
 struct RequestRows {
