@@ -89,3 +89,30 @@ def test_notes_of_spoiled_rows_in_one_workspace(q_lens, lens, prefix, H, KH, D):
         torch.cuda.synchronize()
         assert right(out, bad)
         assert ws[:20].view(torch.int32).tolist()[1:] == [0, 0, 0, 0]  # no status, no count, no note left
+
+
+def test_rows_that_see_only_scores_of_minus_infinity():
+    """exp(-inf) / exp(-inf): such a row is NaN and its log-sum-exp -inf; 0 is for a row that sees no key at all."""
+    nan = float("nan")
+    for q_lens, lens, prefix, D, page, dtype in (
+            ([1, 1, 1], [1, 300, 0], 0, 64, 16, BF), ([1] * 40, [5] * 39 + [0], 0, 128, 16, FP), ([1, 1], [9000, 0], 0, 128, 64, BF),
+            ([40, 3], [40, 2], 0, 128, 16, FP), ([300, 2], [300, 0], 0, 64, 64, BF), ([1] * 30, [0] * 15 + [3] * 15, 700, 128, 16, BF),
+            ([200, 1], [1000, 0], 0, 128, 128, BF), ([3] * 60, [0] * 30 + [40] * 30, 2000, 64, 16, FP)):
+        c = Case(q_lens, lens, prefix, 4, 2, D, page, dtype, seed=17)
+        c.q[..., 5] = c.q[..., 5].abs() + 0.5
+        c.k[..., 5] = -float("inf")
+        got, lse = c.run(return_lse=True)
+        assert bool((lse == -float("inf")).all())
+        cu = c.cu.tolist()
+        for r, length in enumerate(lens):
+            for i in range(q_lens[r]):
+                sees = prefix + max(length - q_lens[r] + i + 1, 0) > 0
+                row = got[cu[r] + i]
+                assert bool((torch.isnan(row) if sees else row == 0).all()), (q_lens, lens, prefix, r, i)
+    # one such key among others has weight 0, and a row that it masks is untouched
+    c = Case([40], [40], 0, 4, 2, 64, 16, BF, seed=18)
+    c.q[..., 5] = c.q[..., 5].abs() + 0.5
+    want = c.run()
+    c.k[int(c.table[0, 0]), :, 0, 5] = -float("inf")
+    got = c.run()
+    assert bool(torch.isnan(got[0]).all()) and bool(torch.isfinite(got[1:]).all()) and not torch.equal(got[1:], want[1:])

@@ -248,7 +248,12 @@ __global__ void __launch_bounds__(256) attention_join_kernel(AttnParams p, AttnP
       }
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  int own = 0;
+  if (l == 0.0f) {
+    const RequestRows rq = request_rows(p, request_of(p.cu_q, d.n_requests, static_cast<int>(n)));
+    own = visible(p, rq, static_cast<int>(n) - rq.q0);
+  }
+  const float inv = reciprocal_sum(p, l, own);
   uint16_t* out = p.out + n * d.out_token_stride + h * d.out_head_stride + lane * kPer;
 #pragma unroll
   for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack16<BF16>(acc[e] * inv, acc[e + 1] * inv);
@@ -330,7 +335,7 @@ __device__ void exact_row(const AttnParams& p, int request, const RequestRows& r
     }
   }
   uint16_t* out = p.out + token * d.out_token_stride + head * d.out_head_stride;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = reciprocal_sum(p, l, seen);
   for (int e = 0; e < D / 32; ++e) out[lane + 32 * e] = narrow16<BF16>(acc[e] * inv);
 }
 

@@ -124,6 +124,14 @@ __device__ __forceinline__ int visible(const AttnParams& p, const RequestRows& x
   return p.d.causal ? max(min(x.len - x.nq + i + 1, x.len), 0) : x.len;
 }
 
+// 1 / l, the sum of a row's weights.  l = 0: a row that sees no key is 0; one whose
+// scores are all -inf is exp(-inf) / exp(-inf), NaN.  (Finite scores make l >= 1.)  own: keys of its
+// request that the row sees.
+__device__ __forceinline__ float reciprocal_sum(const AttnParams& p, float l, int own) {
+  if (l != 0.0f) return 1.0f / l;
+  return own > 0 || p.d.prefix_len > 0 ? __int_as_float(0x7FC00000) : 0.0f;
+}
+
 // The request whose queries include token n: the last r with cu_q[r] <= n.
 __device__ __forceinline__ int request_of(const int32_t* cu_q, int R, int n) {
   int lo = 0, hi = R - 1;

@@ -429,7 +429,7 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
         const float2 ml = __ldcg(p.part_ml + at);
         j.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + e)));
       }
-      const float inv = j.l == 0.0f ? 0.0f : 1.0f / j.l;
+      const float inv = reciprocal_sum(p, j.l, visible(p, rq, row / p.group));
       const uint2 w = make_uint2(pack16<BF16>(j.o.x * inv, j.o.y * inv), pack16<BF16>(j.o.z * inv, j.o.w * inv));
       *reinterpret_cast<uint2*>(p.out + tok * d.out_token_stride + head * d.out_head_stride + e) = w;
       if (p.lse && e == 0) p.lse[grow] = j.l == 0.0f ? -INFINITY : (j.m + log2f(j.l)) * kLn2;

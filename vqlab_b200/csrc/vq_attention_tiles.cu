@@ -609,7 +609,7 @@ attention_tiles_kernel(AttnParams p, AttnPass pass, const __grid_constant__ CUte
         const bool live = g < w.rows;
         const bool partial = pass.part0 >= 0;
         const int64_t at = (pass.part0 + split) * (static_cast<int64_t>(d.n_tokens) * d.heads) + grow;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = reciprocal_sum(p, l, vis);
         // through shared memory (Q's, which no MMA reads any more), so that a row leaves as whole lines: D 16-bit
         // numbers, or half of its fp32 ones at a time
         constexpr int kRowBytes = D * 2, kRowChunks = kRowBytes / 16;
