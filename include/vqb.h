@@ -483,6 +483,9 @@ vqb_status vqb_rotary_append(const vqb_rotary_desc* desc, vqb_dtype dtype, const
  *
  * max_q_len / max_kv_len bound the requests' queries and own tokens (the
  * lengths themselves are on the device): what lies past them is left out.
+ * A query still sees its own place and what lies before it, as far as
+ * max_kv_len goes; rows of queries past max_q_len hold nothing of use.
+ * cu_q[0] is 0.  out overlaps neither q nor the caches.
  * page_size a power of two, 16 to 1024; head_dim 64 or 128; dtype fp16 / bf16;
  * strides in elements, multiples of 8, the elements of a head contiguous; q,
  * caches and out 16-byte aligned.  The first 16 bytes of the workspace are a status

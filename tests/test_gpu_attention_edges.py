@@ -116,3 +116,29 @@ def test_rows_that_see_only_scores_of_minus_infinity():
     c.k[int(c.table[0, 0]), :, 0, 5] = -float("inf")
     got = c.run()
     assert bool(torch.isnan(got[0]).all()) and bool(torch.isfinite(got[1:]).all()) and not torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.parametrize("q_len,H,KH,D,prefix,R", [(5, 6, 2, 64, 0, 3), (5, 6, 2, 128, 300, 3), (40, 8, 2, 64, 50, 3), (40, 8, 2, 128, 0, 3),
+                                                   (300, 4, 1, 128, 0, 2), (12, 4, 2, 64, 0, 80), (20, 8, 2, 128, 700, 80)])
+def test_bounds_below_the_lengths(q_len, H, KH, D, prefix, R):
+    """Keys past max_kv_len are left out, and no other: a query still sees its own place and what lies before it.
+    Queries past max_q_len are left out; those before keep their results."""
+    c = Case([q_len] * R, [500 + r for r in range(R)], prefix, H, KH, D, 16, BF, seed=19)
+    u, G = 2.0 ** -8, H // KH
+    for bound, queries in ((520, q_len), (501, q_len), (500 - q_len // 2, q_len), (500 - q_len, q_len), (64, q_len), (0, q_len), (520, q_len // 2 + 1)):
+        got = c.run(max_kv_len=bound, max_q_len=queries).double()
+        assert torch.equal(got.nan_to_num(7.0), c.run(max_kv_len=bound, max_q_len=queries).double().nan_to_num(7.0)) or queries < q_len
+        for r in (0, R - 1):
+            length = c.lens[r]
+            for h in range(KH):
+                pages = c.table[r, :-(-length // 16)]
+                k, v = (torch.cat([c.rows(x, c.prefix_pages, prefix, h), c.rows(x, pages, length, h)[:bound]]) for x in (c.k, c.v))
+                x = c.q[r * q_len:r * q_len + queries, h * G:(h + 1) * G].double().reshape(-1, D)
+                s = x @ k.T * D ** -0.5
+                last = prefix + length - q_len + torch.arange(queries, device="cuda").repeat_interleave(G)
+                s = s.masked_fill(torch.arange(k.shape[0], device="cuda")[None] > last[:, None], -torch.inf)
+                w = torch.softmax(s, -1) if k.shape[0] else s
+                o, A = w @ v, w @ v.abs()
+                ds = ((x.abs() @ k.abs().T) * D ** 0.5 * 2.0 ** -23 + s.abs().nan_to_num(0, 0, 0) * 2.0 ** -22).amax(-1, keepdim=True) if k.shape[0] else 0.0
+                mine = got[r * q_len:r * q_len + queries, h * G:(h + 1) * G].reshape(-1, D)
+                assert bool(((mine - o).abs() <= u * o.abs() + (u + 2 * ds + 2.0 ** -16) * A + 1e-38).all()), (bound, queries, r, h)

@@ -109,19 +109,22 @@ __device__ __forceinline__ void note_not_finite(const AttnParams& p) { *p.note =
 struct RequestRows {
   int q0;   // first token
   int nq;   // tokens
-  int len;  // keys of its own
+  int len;  // keys of its own that count
+  int at;   // place of its first query among all its keys (below 0: more queries than keys)
 };
 __device__ __forceinline__ RequestRows request_rows(const AttnParams& p, int r) {
   RequestRows x;
-  const int end = min(__ldg(p.cu_q + r + 1), p.d.n_tokens);
+  const int end = __ldg(p.cu_q + r + 1);
   x.q0 = max(__ldg(p.cu_q + r), 0);
-  x.nq = max(end - x.q0, 0);
-  x.len = max(min(__ldg(p.kv_lens + r), p.d.max_kv_len), 0);
+  x.nq = max(min(end, p.d.n_tokens) - x.q0, 0);
+  const int held = max(__ldg(p.kv_lens + r), 0);
+  x.len = min(held, p.d.max_kv_len);
+  x.at = held - max(end - x.q0, 0);
   return x;
 }
 // Own keys that query i of the request sees.
 __device__ __forceinline__ int visible(const AttnParams& p, const RequestRows& x, int i) {
-  return p.d.causal ? max(min(x.len - x.nq + i + 1, x.len), 0) : x.len;
+  return p.d.causal ? max(min(x.at + i + 1, x.len), 0) : x.len;
 }
 
 // 1 / l, the sum of a row's weights.  l = 0: a row that sees no key is 0; one whose

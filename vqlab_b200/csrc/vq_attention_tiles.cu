@@ -240,7 +240,7 @@ __device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& p
     w->request = -1;
     w->rq.q0 = 0;
     w->rq.nq = min(__ldg(p.cu_q + d.n_requests), d.n_tokens);
-    w->rq.len = 0;
+    w->rq.len = w->rq.at = 0;
     w->row0 = block * kRows;
     w->rows = w->rq.nq * p.group;
     w->seg0 = d.prefix_len;
@@ -250,7 +250,7 @@ __device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& p
   int before = 0;
   for (int base = d.n_requests; base > 0; base -= 32) {
     const int r = base - 1 - lane;
-    RequestRows rq{0, 0, 0};
+    RequestRows rq{0, 0, 0, 0};
     if (r >= 0) rq = request_rows(p, r);
     const int pairs = (min(rq.nq, d.max_q_len) * p.group + kRows - 1) / kRows;
     int inc = pairs;
@@ -267,6 +267,7 @@ __device__ __forceinline__ bool find_work(const AttnParams& p, const AttnPass& p
       w->rq.q0 = __shfl_sync(0xffffffffu, rq.q0, src);
       w->rq.nq = __shfl_sync(0xffffffffu, rq.nq, src);
       w->rq.len = __shfl_sync(0xffffffffu, rq.len, src);
+      w->rq.at = __shfl_sync(0xffffffffu, rq.at, src);
       w->rows = min(w->rq.nq, d.max_q_len) * p.group;
       w->row0 = (np - 1 - (block - first)) * kRows;
       w->seg0 = pass.prefix ? d.prefix_len : 0;
