@@ -3,10 +3,13 @@ scores and values that are not finite, bounds below the lengths.
 
 Tolerances are those of test_gpu_prefix_attention.py (derived there, before any run).
 """
+import ctypes
+
 import pytest
 import torch
 
 from test_gpu_prefix_attention import BF, FP, Case
+from vqlab_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +145,26 @@ def test_bounds_below_the_lengths(q_len, H, KH, D, prefix, R):
                 ds = ((x.abs() @ k.abs().T) * D ** 0.5 * 2.0 ** -23 + s.abs().nan_to_num(0, 0, 0) * 2.0 ** -22).amax(-1, keepdim=True) if k.shape[0] else 0.0
                 mine = got[r * q_len:r * q_len + queries, h * G:(h + 1) * G].reshape(-1, D)
                 assert bool(((mine - o).abs() <= u * o.abs() + (u + 2 * ds + 2.0 ** -16) * A + 1e-38).all()), (bound, queries, r, h)
+
+
+@pytest.mark.parametrize("q_len", [1, 4, 40])
+def test_no_block_table(q_len):
+    """A C caller whose requests hold nothing of their own passes no table (max_kv_len 0), whatever its width."""
+    c = Case([q_len] * 9, [0] * 9, 333, 10, 2, 128, 16, BF, seed=21)
+    want = c.run(max_kv_len=0)
+    N = c.q.shape[0]
+    k, v = c.k.stride(), c.v.stride()
+    for width in (0, 7, 4096):
+        d = _lib.AttentionDesc(n_requests=9, n_tokens=N, heads=10, kv_heads=2, head_dim=128, page_size=16, num_pages=c.k.shape[0],
+                               table_width=width, max_q_len=q_len, max_kv_len=0, prefix_len=333, causal=1, scale=128 ** -0.5,
+                               q_token_stride=1280, q_head_stride=128, out_token_stride=1280, out_head_stride=128,
+                               kc_page_stride=k[0], kc_head_stride=k[1], kc_token_stride=k[2], vc_page_stride=v[0],
+                               vc_head_stride=v[1], vc_token_stride=v[2])
+        L, out = _lib.lib(), torch.zeros_like(c.q)
+        ws = torch.empty(L.vqb_prefix_attention_workspace_size(ctypes.byref(d)), dtype=torch.uint8, device="cuda")
+        args = [c.q, c.k, c.v, None, c.kv_lens, c.cu, c.prefix_pages, out, None, ws]
+        ptr = [ctypes.c_void_p(t.data_ptr() if t is not None else None) for t in args]
+        st = L.vqb_prefix_attention(ctypes.byref(d), _lib.VQB_BF16, *ptr, ws.numel(),
+                                    ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert st == _lib.VQB_OK
+        assert torch.equal(out, want)

@@ -154,8 +154,8 @@ attention_decode_kernel(AttnParams p, AttnPass pass, AttnPass shared, const __gr
   if (pass.first) pdl_wait();
   pdl_trigger();
   clear_status(p, pass);
-  // the request's table row is on its way while its lengths are read
-  if (static_cast<int>(threadIdx.x) * 32 < d.table_width)
+  // the request's table row is on its way while its lengths are read (a call whose requests hold nothing may have no table)
+  if (d.max_kv_len > 0 && static_cast<int>(threadIdx.x) * 32 < d.table_width)
     asm volatile("prefetch.global.L1 [%0];"
                  :: "l"(p.table + static_cast<int64_t>(blockIdx.z) * d.table_width + threadIdx.x * 32) : "memory");
 
