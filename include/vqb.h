@@ -408,7 +408,9 @@ vqb_status vqb_ep_reduce(const vqb_ep_layout* layout, void* region, void* y, vqb
  * its turn (the needs of all before it counted), or whose length would pass
  * 2^31 - 1, is refused: its row and its
  * length stay, its new tokens get slot -1, and so does every later one that
- * lacks a page.
+ * lacks a page.  cu_q counts the tokens of a refused request all the same: its
+ * rows of an attention call over these tables are those of queries at the end
+ * of what it held before, and are to be thrown away.
  *
  * Results: block_table_out (unused places -1), kv_lens (tokens held after the
  * step), cu_q [n_requests + 1] (where each request's new tokens start among all

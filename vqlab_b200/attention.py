@@ -48,6 +48,17 @@ class PagedTables(NamedTuple):
     free_pages: torch.Tensor    # int32 [F], the ring of free pages
     state: torch.Tensor         # int64 [4]: start, end, requests refused, 0
 
+    def refused_requests(self) -> torch.Tensor:
+        """bool [R], on the device: requests with new tokens that got no place in
+        this step.  Their tokens (slots -1) are in no cache, and prefix_attention
+        takes their queries for the last of what the request already holds: their
+        rows of its result are to be thrown away, and the tokens given again."""
+        first, end = self.cu_q[:-1], self.cu_q[1:]
+        places = self.slots.numel()
+        if places == 0:
+            return torch.zeros_like(first, dtype=torch.bool)
+        return (end > first) & (first < places) & (self.slots[first.clamp(max=places - 1).long()] < 0)
+
 
 def paged_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
                  free_pages: torch.Tensor, state: torch.Tensor, *, page_size: int, max_tokens: int,
@@ -58,7 +69,9 @@ def paged_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     inplace updates block_table, context_lens (returned as kv_lens), free_pages
     and state; otherwise they are left as they are and new tensors returned
     (state[3] counts the call's blocks meanwhile and is 0 again after it).
-    max_tokens must cover the new tokens; further places are padding."""
+    max_tokens must cover the new tokens; further places are padding.  A request
+    that gets no pages is refused: it keeps what it holds, and its new tokens,
+    which cu_q still counts, have slot -1 (PagedTables.refused_requests)."""
     got = (_lib._native or _lib.native()).paged_tables(context_lens, new_lens, block_table, free_pages, state, page_size,
                                                        max_tokens, position_offset, inplace)
     if type(got) is int:
@@ -176,7 +189,8 @@ class PagedKVCache:
                             inplace=True)
 
     def refused(self) -> int:
-        """Requests that the last step could give no pages (reads the device)."""
+        """How many requests the last step could give no pages (reads the device; its
+        tables' refused_requests says which)."""
         return int(self.state[2])
 
     def share(self, request: int) -> None:
@@ -212,7 +226,8 @@ class VQAttention(torch.nn.Module):
     def forward(self, x: torch.Tensor, cache: PagedKVCache, layer: int, step: PagedTables, max_q_len: int,
                 max_kv_len: int) -> torch.Tensor:
         """x [N, hidden], the step's new tokens in the order of its tables ->
-        [N, hidden].  max_q_len / max_kv_len: the largest new_lens and kv_lens."""
+        [N, hidden].  max_q_len / max_kv_len: the largest new_lens and kv_lens.
+        Rows of a refused request's tokens (step.slots -1) mean nothing."""
         N = x.shape[0]
         q = self.q_proj(x).view(N, self.heads, self.head_dim)
         k = self.k_proj(x).view(N, self.kv_heads, self.head_dim)
