@@ -165,7 +165,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 class PagedKVCache:
     """The key and value pools of a model's layers and one batch's tables over
     them.  `step` builds a step's tables in place; `share` turns what a request
-    holds into the batch's shared prefix."""
+    holds into the batch's shared prefix, `unshare` gives its pages back."""
 
     def __init__(self, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int, max_requests: int,
                  max_context: int, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -205,6 +205,18 @@ class PagedKVCache:
         self.prefix_len = n
         self.block_table[request].fill_(-1)
         self.kv_lens[request] = 0
+
+    def unshare(self) -> None:
+        """Give the shared prefix's pages back (reads the device; no request may hold
+        tokens, whose places follow the prefix's).  Another may then be shared."""
+        _need(self.prefix_len > 0, "the batch has no shared prefix")
+        _need(not any(self.kv_lens.tolist()), "a request holds tokens behind the prefix")
+        n = self.prefix_pages.numel()
+        at = (self.state[1] + torch.arange(n, device=self.state.device)) % self.free_pages.numel()
+        self.free_pages[at] = self.prefix_pages
+        self.state[1] += n
+        self.prefix_pages = None
+        self.prefix_len = 0
 
 
 class VQAttention(torch.nn.Module):
