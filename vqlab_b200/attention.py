@@ -21,6 +21,7 @@ Serving only: no gradients.  CUDA tensors only; fp16 and bf16.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple
 
@@ -153,13 +154,35 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     query that sees nothing gives 0.  max_q_len and max_kv_len bound the
     requests' lengths, which stay on the device.  scale defaults to D ** -0.5.
     Returns [N, heads, D], and with return_lse the fp32 log-sum-exp [N, heads]
-    of the scaled scores; rows past cu_q[-1] are not written."""
+    of the scaled scores; rows past cu_q[-1] are not written.  out must not
+    overlap q or the caches.  workspace: a uint8 tensor that is large enough
+    (attention_workspace), whose first 16 bytes become the call's status block
+    (check_attention); allocated per call when None, and the status is lost then."""
     got = (_lib._native or _lib.native()).prefix_attention(q, k_cache, v_cache, block_table, kv_lens, cu_q, max_q_len,
                                                            max_kv_len, prefix_pages, prefix_len, scale, causal, out,
                                                            return_lse, workspace)
     if type(got) is int:
         _lib.check(got, "vqb_prefix_attention")
     return got
+
+
+def attention_workspace(n_tokens: int, requests: int, heads: int, kv_heads: int, head_dim: int, page_size: int, *,
+                        max_q_len: int, max_kv_len: int, prefix_len: int = 0, device="cuda") -> torch.Tensor:
+    """A workspace for prefix_attention calls of these sizes, for a caller that wants
+    to read a call's status (check_attention); without one a call allocates its own."""
+    d = _lib.AttentionDesc(n_requests=requests, n_tokens=n_tokens, heads=heads, kv_heads=kv_heads, head_dim=head_dim,
+                           page_size=page_size, num_pages=1, table_width=-(-max_kv_len // page_size),
+                           max_q_len=max_q_len, max_kv_len=max_kv_len, prefix_len=prefix_len, scale=1.0)
+    size = int(_lib.lib().vqb_prefix_attention_workspace_size(ctypes.byref(d)))
+    _need(size > 0, "prefix_attention does not take these sizes")
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def check_attention(workspace: torch.Tensor) -> None:
+    """Raise VQBError if a bounded wait on the device gave up in the last
+    prefix_attention call with this workspace, whose result is then incomplete
+    (reads the device).  Every call clears what the one before it left."""
+    _lib.check(int(workspace[4:8].view(torch.int32)), "vqb_prefix_attention")
 
 
 class PagedKVCache:
@@ -236,10 +259,11 @@ class VQAttention(torch.nn.Module):
         self.amplitude, self.interleaved, self.scale = float(amplitude), bool(interleaved), scale
 
     def forward(self, x: torch.Tensor, cache: PagedKVCache, layer: int, step: PagedTables, max_q_len: int,
-                max_kv_len: int) -> torch.Tensor:
+                max_kv_len: int, workspace: torch.Tensor | None = None) -> torch.Tensor:
         """x [N, hidden], the step's new tokens in the order of its tables ->
         [N, hidden].  max_q_len / max_kv_len: the largest new_lens and kv_lens.
-        Rows of a refused request's tokens (step.slots -1) mean nothing."""
+        Rows of a refused request's tokens (step.slots -1) mean nothing.
+        workspace: prefix_attention's."""
         N = x.shape[0]
         q = self.q_proj(x).view(N, self.heads, self.head_dim)
         k = self.k_proj(x).view(N, self.kv_heads, self.head_dim)
@@ -249,5 +273,5 @@ class VQAttention(torch.nn.Module):
                           amplitude=self.amplitude, out=q)
         o = prefix_attention(q, kc, vc, step.block_table, step.kv_lens, step.cu_q, max_q_len=max_q_len,
                              max_kv_len=max_kv_len, prefix_pages=cache.prefix_pages, prefix_len=cache.prefix_len,
-                             scale=self.scale)
+                             scale=self.scale, workspace=workspace)
         return self.o_proj(o.view(N, self.heads * self.head_dim))
