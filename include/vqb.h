@@ -476,12 +476,16 @@ vqb_status vqb_rotary_append(const vqb_rotary_desc* desc, vqb_dtype dtype, const
  * the whole prefix and its own tokens up to kv_lens[r] - n + i (all of them
  * when causal is 0).  Query head h reads key / value head
  * h / (heads / kv_heads).  out = softmax(scale * q k^T) v with scores,
- * softmax and sums in fp32, rounded once to dtype; a row that sees nothing is 0.
+ * softmax and sums in fp32, rounded once to dtype; the softmax's weights are also
+ * rounded to dtype, once, before they meet the values, as the tensor cores need it (up to
+ * half a unit of dtype of sum p |v|); a row that sees nothing is 0.
  * lse (optional, fp32 [n_tokens, heads]): log of the sum of exp of the scaled
  * scores (-inf for such a row).  Rows past cu_q[n_requests] are not written.
  * Cache places past a request's length are never used, whatever they hold; a
  * page outside the pool reads as zeros.  A key or value that is not finite
- * makes the rows that see it what the formula says, and no other.
+ * makes the rows that see it what the formula says, and no other.  Rows from which
+ * the causal mask hides such a value are worked out one by one: a NaN in a prompt's
+ * last value makes the call take up to 90 times as long.
  *
  * max_q_len / max_kv_len bound the requests' queries and own tokens (the
  * lengths themselves are on the device): what lies past them is left out.

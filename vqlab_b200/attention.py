@@ -151,7 +151,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     caches [pages, kv_heads, page_size, D]: first the prefix that all share
     (prefix_len tokens in prefix_pages), then the request's own tokens in the
     pages of its block table row.  Causal within the request's own tokens; a
-    query that sees nothing gives 0.  max_q_len and max_kv_len bound the
+    query that sees nothing gives 0.  Scores, softmax and sums are fp32; the
+    weights are rounded to the caches' type before they meet the values, and the
+    result once.  max_q_len and max_kv_len bound the
     requests' lengths, which stay on the device.  scale defaults to D ** -0.5.
     Returns [N, heads, D], and with return_lse the fp32 log-sum-exp [N, heads]
     of the scaled scores; rows past cu_q[-1] are not written.  out must not

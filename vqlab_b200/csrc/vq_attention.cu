@@ -152,15 +152,20 @@ AttnPlan make_plan(const vqb_attention_desc& d, int sms) {
   a.own.row_tiles = a.decode ? decode_tiles : own_rows / 128;
   if (a.decode) {
     a.own.splits = 1;
-    if (most <= 16 && requests_heads * 8 < sms && keys > 8 * 512) {  // a join kernel pays from about 500 keys a block on
+    // Several clusters a (request, head), of 256 keys a block or more, and a join kernel, where clusters of eight would leave most
+    // SMs idle.  One request with 8 heads at D = 128: 4200 keys 11.7 us, 11.1 in one cluster; 5000 11.8 and 11.9; 6500 12.6 and
+    // 14.1; 8200 12.7 and 16.6; with one head 4200 10.0 and 10.6, 16000 11.4 and 26.3; 8 heads at D = 64: 4200 8.7 and 7.9, 8000 9.5 and 10.0.
+    if (most <= 16 && requests_heads * 8 < sms && keys > 8 * 512) {
       const int64_t fill = ceil_div(2 * sms, requests_heads * 8), most_k = keys / (8 * 256);
       a.own.cluster = 8;
       a.own.splits = static_cast<int>(fill < most_k ? fill : most_k);
     }
     // At D = 64 stages of 32 keys, which share a stage's fixed work: 24 requests of up to 15000 keys 68 -> 62 us, 250 of up
-    // to 5000 214 -> 205 us.  They leave room for three blocks an SM, stages of 16 for four: where that many are one
-    // round (16 requests of up to 2000 keys in 512 blocks: 11.0 against 13.4 us), or run beside the pass over the
-    // prefix (250 of up to 2500 keys behind 9000: 138 against 142 us), stages have 16.
+    // to 5000 214 -> 205 us.  They leave room for three blocks an SM, stages of 16 for four, which is better where that many
+    // blocks are one round and have few keys each, or run beside the pass over the prefix for few; the rule asks for the round
+    // alone.  16 against 32 keys, 8 heads: 74 requests of up to 300 8.6 and 10.9 us, of 2000 33.2 and 32.8; 33 of 2000 18.8 and 20.2; 60 of 1000 17.7
+    // and 16.5; 4 heads: 140 of up to 100 6.0 and 8.9, of 1000 18.2 and 19.0, 117 of 2000 28.9 and 25.6; behind a prefix: 64 of 500
+    // behind 16000 36.5 and 38.5, 30 of 300 behind 3000 12.8 and 14.3, 100 of 1500 behind 5000 49.1 and 45.6, 250 of 2500 behind 9000 145 and 140.
     const int64_t n = requests_heads * a.own.cluster * a.own.splits;
     a.own.stage_keys = d.head_dim == 64 && !joint && !(n > 3 * sms && n <= 4 * sms) ? 32 : 16;
   }
@@ -271,6 +276,8 @@ __device__ __forceinline__ float widen16(uint16_t h) {
 // A row that is not finite, of a request whose later keys it does not see: worked out
 // again, by a warp, over the keys that it does see -- if one of the values that it
 // does not see is indeed not finite.  A row that is not finite by what it sees stays so.
+// Scalar work, for what should not be there: a NaN in the last value of a chunk makes
+// 512 tokens over 1024 keys take 3.1 ms instead of 0.04, 4096 over 8192 24 ms instead of 0.43 (40 heads, D = 128).
 // The log-sum-exp stays as the passes wrote it: it has no values in it.
 template <int D, bool BF16>
 __device__ void exact_row(const AttnParams& p, int request, const RequestRows& rq, int64_t token, int head) {

@@ -7,10 +7,11 @@
 // 2 KB TMA boxes of 16 keys; the warp's first lane refills a stage as soon as the warp has
 // read it), with its own running maximum and sum.  A warp computes
 // S = Q K^T and O += P V with m16n8k16 MMAs: Q and O stay in registers, P goes from
-// the accumulator's layout straight into the next MMA's operand.  Of 17 to 32 rows
+// the accumulator's layout, rounded to the cache's type, straight into the next MMA's operand.  Of 17 to 32 rows
 // two warps take 16 each and share a ring, whose stages are refilled once both have
-// read them.  Long runs of keys move at 6.1 TB/s at D = 128 (24 requests of up to 15000 keys
-// and 5 rows: 112 us); with two row tiles the MMAs begin to bind (24 of up to 8000 and 20 rows: 106 us, 3.7 TB/s).
+// read them.  Long runs of keys move at 6.0 TB/s at D = 128 (24 requests of up to 15000 keys
+// and 5 rows, 8 heads: 115 us; the bytes take 105); with two row tiles the MMAs begin to bind (24 of up to 8000 keys
+// and 20 rows, 4 heads: 66 us, 3.0 TB/s; the bytes take 30).
 //
 // The results are joined without leaving the kernel: the four warps' in shared
 // memory, then the cluster's over distributed shared memory (each block joins its

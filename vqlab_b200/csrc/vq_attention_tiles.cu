@@ -5,7 +5,8 @@
 //
 // A block takes (256 rows of one key/value head and a run of keys): two tiles of
 // 128 rows (a row = a token and a head of the group) that share every K and V
-// tile of 128 keys; or, at D = 64 and for requests of up to 128 rows, one tile.  Roles:
+// tile of 128 keys; or one tile: at D = 64, and at D = 128 for requests of up to 128 rows
+// that are with their heads more than SMs.  Roles:
 //   * a TMA warp fills a ring of shared-memory stages with K and V tiles, one
 //     box a page and 64 elements (a lane a page);
 //   * one thread issues S = Q_t K^T (both from shared memory) into tensor memory,
@@ -23,10 +24,11 @@
 // exponentials and no score waits for a P V.  (With a score tile each, weights
 // had to lie over scores, and each tile's chain of exponentials, P V and Q K^T was
 // serial: 3900 cycles a key tile against 2100 of MMAs.)
-// Bound: the MMAs, at the clock that the power cap leaves: 4096 tokens over up to 8192 keys (40 heads, D = 128) take
-// 463 us, 1.11 PFLOP/s; at D = 64 the exponentials, which take longer than a key tile's MMAs.
+// Bound: the MMAs and the softmax chain between them (2700 cycles a key tile, 2048 of MMAs), at the clock that the power cap
+// leaves: 4096 tokens over up to 8192 keys (40 heads, D = 128) take 428 us as a single call at full clock (1.20
+// PFLOP/s), 468 to 477 us back to back; at D = 64 the exponentials, which take longer than a key tile's MMAs.
 // Scores, weights' sum and O are fp32; the weights are rounded once to the
-// cache's type, which the MMA needs.
+// cache's type, which the MMA needs (their sum takes them as they were).
 //
 // Every wait is bounded (2 s): on expiry the block records VQB_TIMEOUT, waits for
 // its copies and MMAs in flight, frees its tensor memory and returns.
@@ -37,7 +39,7 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 128;
-// NT row tiles a block.  Two (D = 128): one block an SM.  One (D = 64, and at D = 128 requests of up to 128 rows): two
+// NT row tiles a block.  Two (D = 128): one block an SM.  One (D = 64, and at D = 128 where the plan has many small requests): two
 // blocks share an SM, 256 columns of tensor memory each, so that their starts and ends overlap and rows are dealt in 128s.
 // At D = 128 a tile's weights then lie over its scores, the next Q K^T waits for P V, and the other block fills the gaps.
 template <int NT>

@@ -20,7 +20,10 @@
 // the 64-bit remainders, page numbers are products instead of quotients, and
 // rows and tokens are dealt to all SMs.  Per step in a captured graph: 8
 // requests 5.0 -> 3.6 us, 1000 requests with 512-wide rows 9.2 -> 7.6 us (their
-// 5.6 MB take 0.9), 300 prompts of up to 600 tokens 7.2 -> 5.4 us.
+// 5.6 MB take 0.9), 300 prompts of up to 600 tokens 7.2 -> 5.4 us.  In place: 3.3,
+// 9.1 and 6.3 us for steps without new tokens, 13 and 7.9 us for the latter two with
+// (copies that restore the inputs taken off); the arrival of all blocks and the last
+// one's writes are longer than the copies that it saves.
 #include "vqb_common.cuh"
 #include "vqb_internal.h"
 

@@ -3,8 +3,10 @@
 // (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t), t = 2 pi pos f.
 // f is given in turns per position with 64 fraction bits, so pos * f mod 2^64 is
 // the exact fraction of a turn at any position and its upper 32 bits, as a signed
-// number of half turns, go to sincospif: the angle's error is 2^-33 turns where a
-// product of fp32 numbers would lose 2^-24 of a million.
+// number of half turns, go to sincospif.  The lower 32 cost up to 2^-32 turns and the
+// rounding of the upper ones to fp32 up to 2^-26 (half a unit of a number below 1 half
+// turn): 9.5e-8 radians at any position, where a product of fp32 numbers would lose
+// 2^-24 of a million turns.
 //
 // Bound: bytes (each of q, k, v read once and written once).  A block takes a few
 // tokens: it computes their rotary_dim / 2 sines and cosines once into shared
